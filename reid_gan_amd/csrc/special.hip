@@ -78,7 +78,7 @@ __global__ __launch_bounds__(C1_TILE) void conv_c1_fwd_kernel(
     // The weights (and the bias) are indexed by compile-time constants off a kernel argument: they arrive through
     // the scalar cache as SGPR operands of the FMAs (an LDS copy, broadcast-read 144 times per pixel, was what bound
     // an earlier form).  The kernel is bound by vector-instruction issue, so eight of a channel's nine taps run as
-    // four packed FMAs on (tap, tap + 1) pairs - the pairs start at tap 0 for even channels and at tap 1 for odd ones,
+    // four pairs of FMAs on (tap, tap + 1) - the pairs start at tap 0 for even channels and at tap 1 for odd ones,
     // which keeps every weight pair on an even SGPR - and the two half sums are added at the end.
     float acc[8];
     c1_f2 a2[8];                                      // the eight channels' chains side by side, not one after another

@@ -80,7 +80,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 // gmap (NIMG = 2 only, optional): [3][nimg][H][W] partial derivatives of ssim wrt (mu_a, E[aa], E[ar]),
 // i.e. the gradient is taken with respect to image a.
 //
-// The quantities travel as PAIRS so that every filter tap is one v_pk_fma_f32 per pair (the kernel is bound by
+// The quantities travel as PAIRS so that a filter tap treats both of a pair alike (the kernel is bound by
 // vector-instruction issue, not by memory or LDS):
 //   NIMG = 3: (a, b), (aa, bb), (ar, br), (r, rr)        NIMG = 2: (a, r), (aa, rr), (ar, -)
 // and as 16-byte LDS elements: the input tile holds (a, b) pairs [+ a plane of r], the filtered planes hold

@@ -7,7 +7,7 @@ OUT=../libried_gan.so
 FLAGS="-O3 --offload-arch=gfx950 -fPIC -std=c++17 -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops"
 objs=()
 pids=()
-for f in api gemm elementwise special ssim loader legacy attn; do
+for f in api gemm elementwise special ssim loader legacy attn norm rotary xattn xattn_bwd adamw; do
   [ -f $f.hip ] || continue
   stale=0
   [ -f $f.o ] || stale=1

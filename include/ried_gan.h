@@ -475,6 +475,66 @@ int ried_patch_crop(const short* slices_in, const short* slices_tg, int nslices,
 int ried_hu_convert(const void* raw, const double* slope, const int* intercept, short* out, int nslices,
                     long long npix, ried_stream_t stream);
 
+/* ---- token operators: layer norm, rotary positions, cross attention, AdamW over many tensors ------------------------
+ * No counterpart in the reference: the operators of a cross-attention block beside the convolutional path.  Element
+ * types: 0 fp32, 1 bf16, 2 fp16; sums, statistics and softmax are fp32 in registers whatever the type.  Rows and tensors
+ * of layer norm, rotary positions and AdamW may start at any element; cross attention wants 16-byte alignment.
+ *
+ * Layer norm over the last axis of [rows][C] (row strides ldx, ldy in elements): y = (x - mean) * rstd * w + b, w and b
+ * (NULL: left out) fp32 or of the rows' type (wtype); mean, rstd: fp32 [rows] for the backward pass, or NULL.
+ * ried_layer_norm_bwd: dx; dw, db (wtype; NULL: not wanted) = sums over the rows of dy * xh and dy, which need
+ * ried_layer_norm_bwd_scratch_floats() of scratch.  No float atomics: the order of the sums is fixed. */
+int ried_layer_norm_fwd(const void* x, long long ldx, const void* w, const void* b, void* y, long long ldy, float* mean,
+                        float* rstd, long long rows, int C, float eps, int type, int wtype, ried_stream_t stream);
+long long ried_layer_norm_bwd_scratch_floats(long long rows, int C, int type);
+int ried_layer_norm_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* w, const float* mean,
+                        const float* rstd, void* dx, long long lddx, void* dw, void* db, float* scratch, long long rows,
+                        int C, int type, int wtype, ried_stream_t stream);
+/* Rotary positions: x, y [B][L][H][D] (strides xb, xl, xh; channels adjacent; y == x allowed), positions [B][L][axes]
+ * (strides pb, pl, pa; pos_type 0 int32, 1 int64, 2 fp32).  The first s0 pairs turn by the first axis' position, the next
+ * s1 by the second's, and so on; pair j by position * freqs[j] radians (fp64 table of s0 + s1 + s2 + s3 entries).  Pair
+ * j is channels (j, j + pairs), or (2j, 2j + 1) when interleaved; channels behind the pairs pass through.  inverse: by
+ * the negative angle (the backward pass). */
+int ried_rotary(const void* x, long long xb, long long xl, long long xh, void* y, long long yb, long long yl,
+                long long yh, const void* pos, int pos_type, long long pb, long long pl, long long pa,
+                const double* freqs, int s0, int s1, int s2, int s3, int B, int L, int H, int D, int interleaved,
+                int inverse, int type, ried_stream_t stream);
+/* Cross attention: q [batch][queries][heads][dim] over k, v [batch][keys][groups][dim], head h reading key head
+ * h / (heads / groups): o = softmax(scale q k^T) v over the keys j < lengths[b] (NULL: all) with key_mask[b][j] != 0
+ * (NULL: all; one byte per key).  A row without keys gives o = 0, lse = -infinity and no gradient; whatever hidden keys
+ * hold, also NaN, has no effect.  lse [batch][heads][queries]: log of the sum of exp(scores), needed by the backward
+ * pass.  Strides in elements (batch, token, head), channels adjacent; dim a multiple of 8 up to 128, 16-byte alignment,
+ * types 1 and 2.  scratch: as many floats as the size queries say.  The backward pass writes all of dq, dk and dv (zeros
+ * for hidden keys); heads that share a key head are added up in fp32 in a fixed order.
+ * The descriptor is read before the call returns. */
+typedef struct ried_xattn {
+  const void *q, *k, *v;
+  void* o;                                  /* forward: written; backward: read */
+  float* lse;
+  const int* lengths;
+  const unsigned char* key_mask;
+  float* scratch;
+  const void* dout;                         /* backward only, as the next three */
+  void *dq, *dk, *dv;
+  long long q_stride[3], k_stride[3], v_stride[3], o_stride[3], dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+  long long mask_stride, batch, queries, keys, heads, groups, dim, type;
+  double scale;
+} ried_xattn_t;
+long long ried_xattn_fwd_scratch_floats(long long batch, long long queries, long long keys, int heads, int groups, int dim);
+int ried_xattn_fwd(const ried_xattn_t* desc_host, ried_stream_t stream);
+long long ried_xattn_bwd_scratch_floats(long long batch, long long queries, long long keys, int heads, int groups, int dim);
+int ried_xattn_bwd(const ried_xattn_t* desc_host, ried_stream_t stream);
+/* AdamW over many tensors (torch.optim.AdamW's update), moments in 32 or 8 bits.  jobs: device int64 [ntensors][6]: p, m,
+ * v, m scales, v scales (addresses; 0 with 32 bits), elements.  map: device int32 (tensor, chunk) per workgroup of 4096
+ * elements, a tensor's chunks in order, tensor t's first entry at first_host[t] (first_host[ntensors]: their number).
+ * grads_host[t]: gradient of tensor t, of its type (0: no gradient, the tensor is left as it is).  steps: device int32
+ * [ntensors], incremented before use; coef: device fp32 [ntensors][2], scratch.
+ * 8-bit moments: m as e4m3 codes, v as the codes of its square root, a tensor's codes padded to whole blocks of 256
+ * elements (the padding is written as zeros), one fp32 scale per block: value = code * scale. */
+int ried_adamw_jobs(const long long* jobs, const int* map, const long long* grads_host, const int* first_host,
+                    int ntensors, int* steps, float* coef, double lr, double b1, double b2, double eps,
+                    double weight_decay, int type, int state_bits, ried_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

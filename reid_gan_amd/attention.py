@@ -1,0 +1,312 @@
+"""Token operators of a cross-attention block, beside the convolutional path: layer norm, rotary positions of several
+axes, and cross attention to an encoder's states, forward and backward on hand-written kernels.
+
+They have no counterpart in the reference, whose only attention is the Self_Attn layer (src/rinet.py:150-181).
+Tensors live on a ROCm device (there is no CPU path) in fp32, bf16 or fp16 (cross attention: bf16 or fp16); sums,
+statistics and softmax are fp32 whatever the type.  Every call runs on the current stream of its tensors' device and
+allocates what it needs from torch's allocator, so calls on different streams share nothing.
+
+The functions here are differentiable, but their gradients are not made for graph capture: torch's AccumulateGrad nodes
+remember the stream of an earlier eager pass, and a captured backward that meets one ends the process.  A captured
+step calls the forward and backward functions of reid_gan_amd.ops on buffers of its own (as TrainStep does); without
+gradients the functions here may be captured as they are.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Sequence
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+__all__ = ["layer_norm", "LayerNorm", "rotary", "rotary_frequencies", "cross_attention"]
+
+F32 = torch.float32
+
+
+def _check_tensor(what: str, name: str, t, types, device=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: {name} is a tensor, not {type(t).__name__}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{what}: {name} is on {t.device}, not on {device}")
+    if t.dtype not in types:
+        raise TypeError(f"{what}: {name} is {t.dtype}, not one of {', '.join(str(d).replace('torch.', '') for d in types)}")
+
+
+def _on_gpu(what: str, t: torch.Tensor):
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{what}: tensors must be on a ROCm device; there is no CPU path")
+
+
+def _not_captured(what: str):
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what}: gradients are not taken under graph capture; capture the forward and backward "
+                           "functions of reid_gan_amd.ops instead")
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# --------------------------------------------------------------------------- layer norm
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t as [rows][C] with adjacent channels and rows that do not overlap (a copy only where no such view exists)."""
+    C = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, C) if t.dim() > 1 else t.unsqueeze(0)
+    if (C > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < C):
+        t = t.contiguous()
+    if t.stride(0) < C or (C == 1 and t.stride(1) != 1):
+        t = t.as_strided(t.shape, (max(C, t.stride(0)), 1))      # one row, or one channel: strides that nothing uses
+    return t
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        _not_captured("layer_norm")
+        rows = _rows(x)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        mean, rstd = torch.empty(2, rows.shape[0], dtype=F32, device=x.device)
+        ops.layer_norm_fwd(rows, weight, bias, y.view(rows.shape), mean, rstd, eps)
+        ctx.save_for_backward(rows, weight, mean, rstd)
+        ctx.shape, ctx.bias_type = x.shape, None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _not_captured("layer_norm")
+        rows, weight, mean, rstd = ctx.saved_tensors
+        n, C = rows.shape
+        dx = torch.empty(n, C, dtype=rows.dtype, device=rows.device)
+        dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
+        db = torch.empty(C, dtype=ctx.bias_type, device=rows.device) if ctx.needs_input_grad[2] else None
+        scratch = None
+        if dw is not None or db is not None:
+            scratch = torch.empty(ops.layer_norm_bwd_scratch_floats(n, C, rows.dtype), dtype=F32, device=rows.device)
+        ops.layer_norm_bwd(_rows(dy), rows, weight, mean, rstd, dx, dw, db, scratch)
+        return dx.view(ctx.shape) if ctx.needs_input_grad[0] else None, dw, db, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the last axis: (x - mean) / sqrt(var + eps) * weight + bias.
+
+    x: any shape; rows are read where they lie when their channels are adjacent.  weight, bias: [C], contiguous, both fp32
+    or both of x's type, each optional.  The result is contiguous and of x's type; weight and bias gradients are summed
+    in fp32 in a fixed order."""
+    _check_tensor("layer_norm", "x", x, ops.TOKEN_TYPES)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("layer_norm: x has no last axis to normalise")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        _check_tensor("layer_norm", name, t, (F32,) if x.dtype is F32 else (F32, x.dtype), x.device)
+        if t.shape != x.shape[-1:] or not t.is_contiguous():
+            raise ValueError(f"layer_norm: {name} must be a contiguous [{x.shape[-1]}] tensor, not {tuple(t.shape)}")
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
+        raise TypeError("layer_norm: weight and bias have different types")
+    if not eps >= 0:
+        raise ValueError("layer_norm: eps is negative")
+    _on_gpu("layer_norm", x)
+    if _wants_grad(x, weight, bias):
+        return _LayerNormFn.apply(x, weight, bias, float(eps))
+    rows = _rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    ops.layer_norm_fwd(rows, weight, bias, y if y.dim() == 2 else y.view(rows.shape), None, None, float(eps))
+    return y
+
+
+class LayerNorm(torch.nn.Module):
+    """layer_norm with its parameters (names and initialisation of torch.nn.LayerNorm over one axis)."""
+
+    def __init__(self, channels: int, eps: float = 1e-5, elementwise_affine: bool = True, bias: bool = True):
+        super().__init__()
+        self.channels, self.eps = int(channels), eps
+        self.weight = torch.nn.Parameter(torch.ones(self.channels)) if elementwise_affine else None
+        self.bias = torch.nn.Parameter(torch.zeros(self.channels)) if elementwise_affine and bias else None
+
+    def forward(self, x):
+        if x.shape[-1] != self.channels:
+            raise ValueError(f"LayerNorm: {x.shape[-1]} channels, built for {self.channels}")
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+
+# --------------------------------------------------------------------------- rotary positions
+def rotary_frequencies(sections: Sequence[int], base: float = 10000.0, shared: bool = False, device="cuda") -> torch.Tensor:
+    """fp64 table of radians per unit of position, one entry per pair of channels.  Every axis has a ladder of its own,
+    base ** (-j / pairs of the axis); shared: one ladder runs through the sections, base ** (-j / all pairs)."""
+    sections = [int(n) for n in sections]
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) == 0:
+        raise ValueError("rotary_frequencies: sections are the numbers of pairs of one to four axes")
+    ladders = [sum(sections)] if shared else sections
+    return torch.cat([float(base) ** (-torch.arange(n, dtype=torch.float64) / max(n, 1)) for n in ladders]).to(device)
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    def span(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, freqs, sections, interleaved, inverse):
+        _not_captured("rotary")
+        ctx.save_for_backward(positions, freqs)
+        ctx.meta = (sections, interleaved, inverse)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        ops.rotary(x, y, positions, freqs, sections, interleaved, inverse)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _not_captured("rotary")
+        positions, freqs = ctx.saved_tensors
+        sections, interleaved, inverse = ctx.meta
+        if dy.stride(-1) != 1:
+            dy = dy.contiguous()
+        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+        ops.rotary(dy, dx, positions, freqs, sections, interleaved, not inverse)
+        return dx, None, None, None, None, None
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sections: Sequence[int], interleaved: bool = False,
+           inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Turns the channel pairs of x [batch][tokens][heads][channels] by the tokens' positions.
+
+    positions: [batch][tokens][axes] or [tokens][axes], int32, int64 or fp32 (an encoder's coarser grid has positions
+    between the decoder's).  sections: pairs of each axis (slice, row, column ...), one to four; freqs: fp64 table of
+    rotary_frequencies, sum(sections) entries.  Pair j is channels (j, j + pairs), or (2j, 2j + 1) when interleaved;
+    channels behind the pairs pass through.  Angles are formed in 64 bits, so far positions keep their precision.
+    inverse turns back (and is the gradient).  out: where to write, also x itself (no gradients then)."""
+    _check_tensor("rotary", "x", x, ops.TOKEN_TYPES)
+    if x.dim() != 4:
+        raise ValueError("rotary: x is [batch][tokens][heads][channels]")
+    sections = tuple(int(n) for n in sections)
+    pairs = sum(sections)
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or not 0 < 2 * pairs <= x.shape[3]:
+        raise ValueError(f"rotary: sections {sections} do not fit {x.shape[3]} channels (one to four axes, two channels a pair)")
+    _check_tensor("rotary", "positions", positions, ops.POSITION_TYPES, x.device)
+    if positions.dim() == 2:
+        positions = positions.unsqueeze(0).expand(x.shape[0], -1, -1)
+    if positions.shape != (x.shape[0], x.shape[1], len(sections)):
+        raise ValueError(f"rotary: positions are [batch][tokens][{len(sections)}] for x {tuple(x.shape)}, not {tuple(positions.shape)}")
+    _check_tensor("rotary", "freqs", freqs, (torch.float64,), x.device)
+    if freqs.shape != (pairs,) or not freqs.is_contiguous():
+        raise ValueError(f"rotary: freqs is a contiguous table of {pairs} entries")
+    if out is x and x.stride(3) != 1 and x.shape[3] > 1:
+        raise ValueError("rotary: in place needs adjacent channels")
+    if out is None:
+        _on_gpu("rotary", x)
+        if x.stride(3) != 1 and x.shape[3] > 1:
+            x = x.contiguous()
+        if _wants_grad(x):
+            return _RotaryFn.apply(x, positions, freqs, sections, bool(interleaved), bool(inverse))
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        if _wants_grad(x, out):
+            raise RuntimeError("rotary: out= has no gradient; leave it out, or use torch.no_grad()")
+        _check_tensor("rotary", "out", out, (x.dtype,), x.device)
+        if out.shape != x.shape or (out.stride(3) != 1 and out.shape[3] > 1):
+            raise ValueError("rotary: out has x's shape and adjacent channels")
+        if any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride())):
+            raise ValueError("rotary: out is an expanded tensor")
+        same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
+        if not same and x.numel() and (_overlap(out, x) or _overlap(out, positions)):
+            raise ValueError("rotary: out overlaps x or positions without being x")
+        _on_gpu("rotary", x)
+        if x.stride(3) != 1 and x.shape[3] > 1:
+            x = x.contiguous()
+    ops.rotary(x, out, positions, freqs, sections, bool(interleaved), bool(inverse))
+    return out
+
+
+# --------------------------------------------------------------------------- cross attention
+def _laid_out(t: torch.Tensor) -> torch.Tensor:
+    """t [batch][tokens][heads][channels] as the kernels read it: adjacent channels, strides in multiples of 8 elements,
+    16-byte alignment (a copy only where it is not)."""
+    s = t.stride()
+    if s[3] == 1 and not (s[0] | s[1] | s[2]) & 7 and s[0] >= 0 and 0 <= s[1] <= 1 << 23 and s[2] >= 0 and not t.data_ptr() & 15:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _attend(q, k, v, lengths, key_mask, scale, lse):
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    n = ops.xattn_fwd_scratch_floats(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3])
+    scratch = torch.empty(n, dtype=F32, device=q.device) if n else None
+    ops.xattn_fwd(q, k, v, out, lse, scale, lengths, key_mask, scratch)
+    return out
+
+
+class _CrossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, key_mask, scale):
+        _not_captured("cross_attention")
+        q, k, v = _laid_out(q), _laid_out(k), _laid_out(v)
+        lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=F32, device=q.device)
+        out = _attend(q, k, v, lengths, key_mask, scale, lse)
+        ctx.save_for_backward(q, k, v, out, lse, lengths, key_mask)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        _not_captured("cross_attention")
+        q, k, v, out, lse, lengths, key_mask = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        if q.shape[1] == 0:
+            return dq, dk.zero_(), dv.zero_(), None, None, None
+        n = ops.xattn_bwd_scratch_floats(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3])
+        scratch = torch.empty(n, dtype=F32, device=q.device)
+        ops.xattn_bwd(_laid_out(dout), q, k, v, out, lse, dq, dk, dv, ctx.scale, scratch, lengths, key_mask)
+        return dq, dk, dv, None, None, None
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tensor] = None,
+                    key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """softmax(scale q k^T) v of queries [batch][queries][heads][channels] over an encoder's states k, v
+    [batch][keys][key heads][channels], of any other length.
+
+    Head h reads key head h // (heads // key heads).  lengths: int32 [batch], the first so many keys of each entry
+    count; key_mask: bool or uint8 [batch][keys], nonzero keys count; with both, keys that both allow.  An entry without
+    keys gives zeros and no gradient; hidden keys have no effect whatever they hold, and get zero gradients.  scale:
+    channels ** -0.5 unless given.  channels: a multiple of 8 up to 128, bf16 or fp16.  Views are read where they lie when
+    their channels are adjacent and their strides are multiples of 8 elements; others are copied."""
+    types = (torch.bfloat16, torch.float16)
+    _check_tensor("cross_attention", "q", q, types)
+    _check_tensor("cross_attention", "k", k, (q.dtype,), q.device)
+    _check_tensor("cross_attention", "v", v, (q.dtype,), q.device)
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"cross_attention: q [batch][queries][heads][channels] and k, v [batch][keys][key heads][channels] do "
+                         f"not fit: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, Lq, H, D = q.shape
+    if H == 0 or k.shape[2] == 0 or H % k.shape[2]:
+        raise ValueError(f"cross_attention: {H} heads do not divide over {k.shape[2]} key heads")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"cross_attention: {D} channels are not a multiple of 8 up to 128")
+    if lengths is not None:
+        _check_tensor("cross_attention", "lengths", lengths, (torch.int32,), q.device)
+        if lengths.shape != (B,) or not lengths.is_contiguous():
+            raise ValueError(f"cross_attention: lengths is a contiguous [{B}] tensor")
+    if key_mask is not None:
+        _check_tensor("cross_attention", "key_mask", key_mask, (torch.bool, torch.uint8), q.device)
+        if key_mask.shape != (B, k.shape[1]):
+            raise ValueError(f"cross_attention: key_mask is [{B}][{k.shape[1]}], not {tuple(key_mask.shape)}")
+        if key_mask.stride(0) < 0 or (key_mask.stride(1) != 1 and key_mask.shape[1] > 1):
+            key_mask = key_mask.contiguous()
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < 1e30 or math.isnan(scale):
+        raise ValueError("cross_attention: scale is a positive number")
+    _on_gpu("cross_attention", q)
+    if _wants_grad(q, k, v):
+        return _CrossFn.apply(q, k, v, lengths, key_mask, scale)
+    return _attend(_laid_out(q), _laid_out(k), _laid_out(v), lengths, key_mask, scale, None)

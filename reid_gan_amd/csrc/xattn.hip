@@ -1,0 +1,469 @@
+// Cross attention to an encoder's states, forward:  S = scale q k^T over the keys that count, P = softmax S, o = P v.
+// A row without keys gives zeros (and a log-sum of -infinity).
+//
+// Heads that share a key head are folded into its rows (row = head in group * queries + query), so that a tile of keys
+// and values serves them all.
+#include "xattn.h"
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Tiles: a block of four waves owns 128 rows, a wave 32; tiles of 64 keys go HBM -> LDS by DMA, two stages, one barrier
+// per tile.  S^T = K Q^T leaves a row's scores in one lane pair, so the softmax runs in registers, and P^T is the B operand
+// of O^T += V^T P^T as it stands.  The running maximum is raised only when a score exceeds it by more than 2^8 (the
+// sums hold that in fp32): rescaling is rare after the first tile.
+// ---------------------------------------------------------------------------------------------------------------------
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaArgs A) {
+  constexpr int KS = XaTile<DP>::KS, DT = XaTile<DP>::DT, RB = XaTile<DP>::RB, NC = XaTile<DP>::NC, RPI = XaTile<DP>::RPI;
+  constexpr int TILE = 64 * RB, NI = 16 / RPI;                    // DMA instructions per wave and operand
+  extern __shared__ __align__(16) char smem[];                    // [2][K tile, V tile]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  int inner, head;
+  xa_block(A.tiles * A.nsplit, A.B * A.Hkv, inner, head);
+  const int b = head / A.Hkv, hk = head % A.Hkv, tile = inner % A.tiles, split = inner / A.tiles;
+  const int row = tile * 128 + wave * 32 + (lane & 31);
+  const bool live = row < A.rows;
+  const int g = live ? row / A.Lq : 0, qi = live ? row - g * A.Lq : 0;
+  const T* qp = (const T*)A.q + (long long)b * A.qs[0] + (long long)qi * A.qs[1] + (long long)(hk * A.G + g) * A.qs[2];
+  u32x4 fq[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d = s * 16 + h * 8;
+    fq[s] = live && d < A.D ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{0, 0, 0, 0};
+  }
+  const int nk = xa_keys(A, b), ntile = (nk + 63) >> 6, per = (ntile + A.nsplit - 1) / A.nsplit;
+  const int t0 = split * per, t1 = t0 + per < ntile ? t0 + per : ntile;
+  const char* kp = (const char*)((const T*)A.k + (long long)b * A.ks[0] + (long long)hk * A.ks[2]);
+  const char* vp = (const char*)((const T*)A.v + (long long)b * A.vs[0] + (long long)hk * A.vs[2]);
+  const unsigned char* mp = A.mask ? A.mask + (long long)b * A.ms : nullptr;
+  const int krow = (int)A.ks[1] * 2, vrow = (int)A.vs[1] * 2;    // bytes (host-checked: 64 rows stay below 2^31)
+  const int srow = wave * RPI + lane / NC, sc = (lane % NC) ^ xa_swz(srow);
+  const unsigned dead = sc * 8 >= A.D ? XA_OOB : 0u;
+  const unsigned koff = (unsigned)(srow * krow + sc * 16) | dead, voff = (unsigned)(srow * vrow + sc * 16) | dead;
+  auto issue = [&](int t, u64 w, int buf) {
+    const __amdgpu_buffer_rsrc_t rk = xa_rsrc(kp + (long long)t * 64 * krow), rv = xa_rsrc(vp + (long long)t * 64 * vrow);
+    char* dst = smem + buf * 2 * TILE + wave * RPI * RB;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const unsigned bad = (w >> (srow + i * 4 * RPI)) & 1 ? 0u : XA_OOB;
+      xa_dma16(rk, koff | bad, i * 4 * RPI * krow, dst + i * 4 * RPI * RB);
+      xa_dma16(rv, voff | bad, i * 4 * RPI * vrow, dst + TILE + i * 4 * RPI * RB);
+    }
+  };
+  auto mask_byte = [&](int t) -> int {
+    const int key = t * 64 + lane;
+    return mp && key < nk ? mp[key] : 0;
+  };
+  const float c = A.scale * XA_LOG2E;
+  float m = -INFINITY, mc = 0.f, sum = 0.f;
+  f32x16 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = xa_zero();
+
+  u64 w = 0;
+  int byte = 0, buf = 0;
+  if (t0 < t1) {
+    w = xa_word(nk - t0 * 64, mp != nullptr, mask_byte(t0));
+    issue(t0, w, 0);
+    byte = mask_byte(t0 + 1);
+  }
+  for (int t = t0; t < t1; ++t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();                                 // tile t has landed; everyone is done with the other stage
+    asm volatile("" ::: "memory");
+    u64 wn = 0;
+    if (t + 1 < t1) {
+      wn = xa_word(nk - (t + 1) * 64, mp != nullptr, byte);
+      issue(t + 1, wn, buf ^ 1);
+      byte = mask_byte(t + 2);
+    }
+    if (w) {
+      const char* kt = smem + buf * 2 * TILE;
+      const char* vt = kt + TILE;
+      f32x16 s[2] = {xa_zero(), xa_zero()};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) s[u] = xa_mma<T>(xa_frag<DP>(kt, 32 * u, ks, lane), fq[ks], s[u]);
+      if (w != ~0ull) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const unsigned bits = (unsigned)(w >> (32 * u)) >> (4 * h);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[u][r] = (bits >> (8 * (r >> 2) + (r & 3))) & 1 ? s[u][r] : -INFINITY;
+        }
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
+      if (__any((mx - m) * c > 8.f || (m == -INFINITY && mx > m))) {
+        float lo, hi;
+        xa_halves(mx, lo, hi);
+        const float mn = fmaxf(m, fmaxf(lo, hi));
+        const float nc = mn == -INFINITY ? 0.f : mn * c;
+        const float a = xa_exp2((m == -INFINITY ? -INFINITY : mc) - nc);
+        m = mn;
+        mc = nc;
+        sum *= a;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] *= a;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[u][r] = xa_exp2(__builtin_fmaf(s[u][r], c, -mc));
+          sum += s[u][r];
+        }
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+        const u32x4 p = xa_as_b<T>(s[kb >> 1], kb & 1);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(xa_tr_frag<DP>(vt, kb * 16, d, lane), p, acc[d]);
+      }
+    }
+    w = wn;
+    buf ^= 1;
+  }
+  float lo, hi;
+  xa_halves(sum, lo, hi);
+  const float total = lo + hi;
+  // (zero only for a row without keys: a row's largest weight is at least 1.  NaN goes on to the result.)
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const float lse = total == 0.f ? -INFINITY : (mc + __log2f(total)) * XA_LN2;
+  if (!live) return;
+  const long long flat = (long long)head * A.rows + row;
+  if (A.nsplit == 1) {
+    if (h == 0 && A.lse) A.lse[flat] = lse;
+    T* op = (T*)A.out + (long long)b * A.os[0] + (long long)qi * A.os[1] + (long long)(hk * A.G + g) * A.os[2];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int ch = d * 32 + 2 * r + 4 * h;
+        if (ch < A.D)
+          *reinterpret_cast<u32x2*>(op + ch) = u32x2{xa_pack<T>(acc[d][r] * inv, acc[d][r + 1] * inv),
+                                                     xa_pack<T>(acc[d][r + 2] * inv, acc[d][r + 3] * inv)};
+      }
+  } else {
+    const long long at = (long long)split * A.B * A.Hkv * A.rows + flat;
+    if (h == 0) A.part_lse[at] = lse;
+    float* op = A.part + at * A.D;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int ch = d * 32 + 2 * r + 4 * h;
+        if (ch < A.D)
+          *reinterpret_cast<f32x4*>(op + ch) = f32x4{acc[d][r] * inv, acc[d][r + 1] * inv, acc[d][r + 2] * inv, acc[d][r + 3] * inv};
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Few rows (up to 32 per key head: single tokens): the four waves of a block take turns at tiles of 32 keys of the block's
+// share of the keys, each with two DMA stages of its own (no barrier in the loop), and are joined through LDS.
+// ---------------------------------------------------------------------------------------------------------------------
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 1) void xattn_token_kernel(XaArgs A) {
+  constexpr int KS = XaTile<DP>::KS, DT = XaTile<DP>::DT, RB = XaTile<DP>::RB, NC = XaTile<DP>::NC, RPI = XaTile<DP>::RPI;
+  constexpr int TILE = 32 * RB, NI = 32 / RPI, PO = DP + 4;       // PO: row pitch (floats) of the exchange
+  static_assert(4 * (32 * PO + 64) * 4 <= 4 * 2 * 2 * TILE, "the exchange reuses the stages");
+  extern __shared__ __align__(16) char smem[];                    // [4 waves][2 stages][K tile, V tile]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  int split, head;
+  xa_block(A.nsplit, A.B * A.Hkv, split, head);
+  const int b = head / A.Hkv, hk = head % A.Hkv, row = lane & 31;
+  const bool live = row < A.rows;
+  const int g = live ? row / A.Lq : 0, qi = live ? row - g * A.Lq : 0;
+  const T* qp = (const T*)A.q + (long long)b * A.qs[0] + (long long)qi * A.qs[1] + (long long)(hk * A.G + g) * A.qs[2];
+  u32x4 fq[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d = s * 16 + h * 8;
+    fq[s] = live && d < A.D ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{0, 0, 0, 0};
+  }
+  const int nk = xa_keys(A, b), ntile = (nk + 31) >> 5, per = (ntile + A.nsplit - 1) / A.nsplit;
+  const int t0 = split * per + wave, t1 = split * per + per < ntile ? split * per + per : ntile;
+  const char* kp = (const char*)((const T*)A.k + (long long)b * A.ks[0] + (long long)hk * A.ks[2]);
+  const char* vp = (const char*)((const T*)A.v + (long long)b * A.vs[0] + (long long)hk * A.vs[2]);
+  const unsigned char* mp = A.mask ? A.mask + (long long)b * A.ms : nullptr;
+  const int krow = (int)A.ks[1] * 2, vrow = (int)A.vs[1] * 2;
+  const int srow = lane / NC;
+  char* const base = smem + wave * 4 * TILE;
+  // (a wave's DMA instruction i fills rows i * RPI ..; with RPI = 4 the swizzle of odd i differs)
+  auto issue = [&](int t, unsigned w, int buf) {
+    const __amdgpu_buffer_rsrc_t rk = xa_rsrc(kp + (long long)t * 32 * krow), rv = xa_rsrc(vp + (long long)t * 32 * vrow);
+    char* dst = base + buf * 2 * TILE;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = srow + i * RPI, sc = (lane % NC) ^ xa_swz(r);
+      const unsigned bad = ((w >> r) & 1) && sc * 8 < A.D ? 0u : XA_OOB;
+      xa_dma16(rk, (unsigned)(srow * krow + sc * 16) | bad, i * RPI * krow, dst + i * RPI * RB);
+      xa_dma16(rv, (unsigned)(srow * vrow + sc * 16) | bad, i * RPI * vrow, dst + TILE + i * RPI * RB);
+    }
+  };
+  auto mask_byte = [&](int t) -> int {
+    const int key = t * 32 + (lane & 31);
+    return mp && key < nk ? mp[key] : 0;
+  };
+  auto word = [&](int t, int byte) -> unsigned {
+    return t < t1 ? (unsigned)xa_word(nk - t * 32, mp != nullptr, byte) : 0u;
+  };
+  const float c = A.scale * XA_LOG2E;
+  float m = -INFINITY, mc = 0.f, sum = 0.f;
+  f32x16 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = xa_zero();
+  if (t0 < t1) {
+    int byte = mask_byte(t0), byte1 = mask_byte(t0 + 4);
+    unsigned w = word(t0, byte), w1 = word(t0 + 4, byte1);
+    issue(t0, w, 0);
+    byte = mask_byte(t0 + 8);
+    issue(t0 + 4 < t1 ? t0 + 4 : t0, w1, 1);                      // (past the end: zeros, so that the count holds)
+    int buf = 0;
+    for (int t = t0; t < t1; t += 4) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
+      const char* kt = base + buf * 2 * TILE;
+      const char* vt = kt + TILE;
+      f32x16 s = xa_zero();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s = xa_mma<T>(xa_frag<DP>(kt, 0, ks, lane), fq[ks], s);
+      if ((w & 0xffffffffu) != 0xffffffffu) {
+        const unsigned bits = w >> (4 * h);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = (bits >> (8 * (r >> 2) + (r & 3))) & 1 ? s[r] : -INFINITY;
+      }
+      float mx = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+      if (__any((mx - m) * c > 8.f || (m == -INFINITY && mx > m))) {
+        float lo, hi;
+        xa_halves(mx, lo, hi);
+        const float mn = fmaxf(m, fmaxf(lo, hi));
+        const float nc = mn == -INFINITY ? 0.f : mn * c;
+        const float a = xa_exp2((m == -INFINITY ? -INFINITY : mc) - nc);
+        m = mn;
+        mc = nc;
+        sum *= a;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] *= a;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = xa_exp2(__builtin_fmaf(s[r], c, -mc));
+        sum += s[r];
+      }
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const u32x4 p = xa_as_b<T>(s, kb);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(xa_tr_frag<DP>(vt, kb * 16, d, lane), p, acc[d]);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // this stage has been read
+      const unsigned w2 = word(t + 8, byte);
+      byte = mask_byte(t + 12);
+      issue(t + 8 < t1 ? t + 8 : t0, w2, buf);
+      w = w1;
+      w1 = w2;
+      buf ^= 1;
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                // no DMA may land in the exchange
+  __syncthreads();
+  float* ex = reinterpret_cast<float*>(smem) + wave * (32 * PO + 64);
+  {
+    float lo, hi;
+    xa_halves(sum, lo, hi);
+    if (h == 0) {
+      ex[32 * PO + row] = m == -INFINITY ? -INFINITY : mc;
+      ex[32 * PO + 32 + row] = lo + hi;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<f32x4*>(ex + row * PO + d * 32 + 2 * r + 4 * h) = f32x4{acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]};
+  }
+  __syncthreads();
+  const float* e0 = reinterpret_cast<const float*>(smem);
+  for (int i = tid; i < A.rows * (DP / 4); i += 256) {
+    const int r = i / (DP / 4), d = (i % (DP / 4)) * 4;
+    float top = -INFINITY, tot = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float mk = e0[k * (32 * PO + 64) + 32 * PO + r];
+      top = mk > top || mk != mk ? mk : top;
+    }
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float* e = e0 + k * (32 * PO + 64);
+      const float mk = e[32 * PO + r], f = mk == -INFINITY ? 0.f : xa_exp2(mk - top);
+      tot += e[32 * PO + 32 + r] * f;
+      o += *reinterpret_cast<const f32x4*>(e + r * PO + d) * f;
+    }
+    const float inv = tot == 0.f ? 0.f : 1.f / tot;
+    const float lse = tot == 0.f ? -INFINITY : (top + __log2f(tot)) * XA_LN2;
+    const long long flat = (long long)head * A.rows + r;
+    o *= inv;
+    if (A.nsplit == 1) {
+      const int gg = r / A.Lq, qq = r - gg * A.Lq;
+      if (d == 0 && A.lse) A.lse[flat] = lse;
+      if (d < A.D)
+        *reinterpret_cast<u32x2*>((T*)A.out + (long long)b * A.os[0] + (long long)qq * A.os[1] +
+                                  (long long)(hk * A.G + gg) * A.os[2] + d) = u32x2{xa_pack<T>(o[0], o[1]), xa_pack<T>(o[2], o[3])};
+    } else {
+      const long long at = (long long)split * A.B * A.Hkv * A.rows + flat;
+      if (d == 0) A.part_lse[at] = lse;
+      if (d < A.D) *reinterpret_cast<f32x4*>(A.part + at * A.D + d) = o;
+    }
+  }
+}
+
+// joins the shares of the keys: a thread per row and 8 channels
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs A) {
+  const int chunks = A.D >> 3;
+  const long long all = (long long)A.B * A.Hkv * A.rows, i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= all * chunks) return;
+  const long long flat = i / chunks;
+  const int d = (int)(i - flat * chunks) * 8;
+  float top = -INFINITY;
+  for (int s = 0; s < A.nsplit; ++s) {
+    const float l = A.part_lse[s * all + flat];
+    top = l > top || l != l ? l : top;
+  }
+  float o[8] = {}, tot = 0.f;
+  for (int s = 0; s < A.nsplit; ++s) {
+    const float l = A.part_lse[s * all + flat], f = l == -INFINITY ? 0.f : xa_exp2((l - top) * XA_LOG2E);
+    const float* p = A.part + (s * all + flat) * A.D + d;
+    tot += f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] += f == 0.f ? 0.f : p[k] * f;
+  }
+  const float inv = tot == 0.f ? 0.f : 1.f / tot;
+  const int head = (int)(flat / A.rows), row = (int)(flat - (long long)head * A.rows);
+  const int b = head / A.Hkv, hk = head % A.Hkv, g = row / A.Lq, qi = row - g * A.Lq;
+  if (d == 0 && A.lse) A.lse[flat] = tot == 0.f ? -INFINITY : top + __logf(tot);
+  T* op = (T*)A.out + (long long)b * A.os[0] + (long long)qi * A.os[1] + (long long)(hk * A.G + g) * A.os[2] + d;
+  *reinterpret_cast<u32x4*>(op) = u32x4{xa_pack<T>(o[0] * inv, o[1] * inv), xa_pack<T>(o[2] * inv, o[3] * inv),
+                                        xa_pack<T>(o[4] * inv, o[5] * inv), xa_pack<T>(o[6] * inv, o[7] * inv)};
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------------
+struct XaSplit { int tiles, nsplit; };
+// Shares of the keys per block row: the forward kernels want 512 blocks (two per CU, one for single tokens at D > 64);
+// a share keeps at least 4 tiles per wave that reads it.
+static XaSplit xa_fwd_split(const ried_xattn_t& d) {
+  const long long rows = d.heads / d.groups * d.queries, heads = d.batch * d.groups;
+  XaSplit s;
+  s.tiles = rows <= 32 ? 1 : ceil_div(rows, 128);
+  const long long blocks = s.tiles * heads;
+  const long long want = rows <= 32 && d.dim > 64 ? 256 : 512, most = rows <= 32 ? d.keys / 512 : d.keys / 256;
+  long long n = want / (blocks > 0 ? blocks : 1);
+  if (n > most) n = most;
+  if (n > 64) n = 64;
+  s.nsplit = n < 1 ? 1 : (int)n;
+  return s;
+}
+
+int xa_check(const ried_xattn_t* d, const char* name, bool bwd) {
+  RIED_CHECK_ARG(d, "%s: null descriptor", name);
+  RIED_CHECK_ARG(d->type == RIED_T_BF16 || d->type == RIED_T_F16, "%s: types are 1 bf16, 2 fp16", name);
+  RIED_CHECK_ARG(d->batch >= 0 && d->queries >= 0 && d->keys >= 0 && d->heads > 0 && d->groups > 0 && d->heads % d->groups == 0,
+                 "%s: bad sizes (batch %lld, queries %lld, keys %lld, heads %lld over %lld key heads)", name, d->batch,
+                 d->queries, d->keys, d->heads, d->groups);
+  RIED_CHECK_ARG(d->dim >= 8 && d->dim <= 128 && d->dim % 8 == 0, "%s: head dimension %lld is not a multiple of 8 up to 128", name, d->dim);
+  RIED_CHECK_ARG(d->keys <= (1ll << 30) && d->queries <= (1ll << 30) && d->batch <= (1ll << 20) && d->heads <= (1ll << 20) &&
+                 d->heads / d->groups * d->queries <= (1ll << 30) && d->batch * d->groups <= (1ll << 24),
+                 "%s: sizes out of range", name);
+  RIED_CHECK_ARG(d->scale > 0 && d->scale < 1e30, "%s: the scale is a positive number", name);
+  if (d->batch == 0 || d->queries == 0) return RIED_OK;
+  struct View { const void* p; const long long* s; const char* n; bool need; } views[] = {
+      {d->q, d->q_stride, "q", true}, {d->k, d->k_stride, "k", d->keys > 0}, {d->v, d->v_stride, "v", d->keys > 0},
+      {d->o, d->o_stride, "o", true}, {d->dout, d->dout_stride, "dout", bwd}, {d->dq, d->dq_stride, "dq", bwd},
+      {d->dk, d->dk_stride, "dk", bwd && d->keys > 0}, {d->dv, d->dv_stride, "dv", bwd && d->keys > 0}};
+  for (const View& v : views) {
+    if (!v.need) continue;
+    RIED_CHECK_ARG(v.p && ((uintptr_t)v.p & 15) == 0, "%s: %s is null or not 16-byte aligned", name, v.n);
+    for (int i = 0; i < 3; ++i)
+      RIED_CHECK_ARG(v.s[i] >= 0 && v.s[i] % 8 == 0, "%s: strides of %s are multiples of 8 elements", name, v.n);
+    RIED_CHECK_ARG(v.s[1] <= (1 << 23), "%s: token stride of %s is over 2^23 elements", name, v.n);
+  }
+  return RIED_OK;
+}
+
+XaArgs xa_args(const ried_xattn_t& d) {
+  XaArgs A = {};
+  A.q = d.q; A.k = d.k; A.v = d.v; A.o = d.o; A.out = d.o; A.dout = d.dout; A.dq = d.dq; A.dk = d.dk; A.dv = d.dv;
+  A.lse = d.lse; A.lengths = d.lengths; A.mask = d.key_mask; A.ms = d.mask_stride;
+  for (int i = 0; i < 3; ++i) {
+    A.qs[i] = d.q_stride[i]; A.ks[i] = d.k_stride[i]; A.vs[i] = d.v_stride[i]; A.os[i] = d.o_stride[i];
+    A.gs[i] = d.dout_stride[i]; A.dqs[i] = d.dq_stride[i]; A.dks[i] = d.dk_stride[i]; A.dvs[i] = d.dv_stride[i];
+  }
+  A.B = (int)d.batch; A.Lq = (int)d.queries; A.Lk = (int)d.keys; A.Hkv = (int)d.groups; A.G = (int)(d.heads / d.groups);
+  A.D = (int)d.dim; A.rows = A.G * A.Lq; A.scale = (float)d.scale;
+  return A;
+}
+
+extern "C" long long ried_xattn_fwd_scratch_floats(long long batch, long long queries, long long keys, int heads,
+                                                   int groups, int dim) {
+  if (batch <= 0 || queries <= 0 || heads <= 0 || groups <= 0 || heads % groups) return 0;
+  ried_xattn_t d = {};
+  d.batch = batch; d.queries = queries; d.keys = keys; d.heads = heads; d.groups = groups; d.dim = dim;
+  const XaSplit s = xa_fwd_split(d);
+  return s.nsplit == 1 ? 0 : s.nsplit * batch * heads * queries * (dim + 1);
+}
+
+template <typename K>
+static int xa_lds(K kernel, int bytes, const char* name) {
+  const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  RIED_CHECK_ARG(e == hipSuccess, "%s: %d bytes of LDS: %s", name, bytes, hipGetErrorString(e));
+  return RIED_OK;
+}
+
+template <typename T, int DP>
+static int xa_fwd_launch(const XaArgs& A, hipStream_t stream) {
+  const unsigned grid = (unsigned)(A.tiles * A.nsplit * A.B * A.Hkv);
+  if (A.rows <= 32) {
+    constexpr int lds = 4 * 2 * 2 * 32 * XaTile<DP>::RB;
+    if (int e = xa_lds(xattn_token_kernel<T, DP>, lds, "ried_xattn_fwd")) return e;
+    hipLaunchKernelGGL((xattn_token_kernel<T, DP>), dim3(grid), dim3(256), lds, stream, A);
+  } else {
+    constexpr int lds = 2 * 2 * 64 * XaTile<DP>::RB;
+    if (int e = xa_lds(xattn_fwd_kernel<T, DP>, lds, "ried_xattn_fwd")) return e;
+    hipLaunchKernelGGL((xattn_fwd_kernel<T, DP>), dim3(grid), dim3(256), lds, stream, A);
+  }
+  if (A.nsplit > 1)
+    hipLaunchKernelGGL((xattn_join_kernel<T>), dim3(ceil_div((long long)A.B * A.Hkv * A.rows * (A.D >> 3), 256)), dim3(256), 0, stream, A);
+  return RIED_OK;
+}
+template <typename T>
+static int xa_fwd_dim(const XaArgs& A, hipStream_t stream) {
+  return A.D <= 32 ? xa_fwd_launch<T, 32>(A, stream) : A.D <= 64 ? xa_fwd_launch<T, 64>(A, stream)
+       : A.D <= 96 ? xa_fwd_launch<T, 96>(A, stream) : xa_fwd_launch<T, 128>(A, stream);
+}
+
+extern "C" int ried_xattn_fwd(const ried_xattn_t* desc, hipStream_t stream) {
+  if (int e = xa_check(desc, "ried_xattn_fwd", false)) return e;
+  const ried_xattn_t& d = *desc;
+  if (d.batch == 0 || d.queries == 0) return RIED_OK;
+  XaArgs A = xa_args(d);
+  const XaSplit s = xa_fwd_split(d);
+  A.tiles = s.tiles;
+  A.nsplit = s.nsplit;
+  RIED_CHECK_ARG((long long)A.tiles * A.nsplit * A.B * A.Hkv <= 0x7fffffffll, "ried_xattn_fwd: too many blocks");
+  if (A.nsplit > 1) {
+    RIED_CHECK_ARG(d.scratch, "ried_xattn_fwd: this call needs ried_xattn_fwd_scratch_floats() of scratch");
+    A.part = d.scratch;
+    A.part_lse = d.scratch + (long long)A.nsplit * A.B * A.Hkv * A.rows * A.D;
+  }
+  const int e = d.type == RIED_T_BF16 ? xa_fwd_dim<bf16_t>(A, stream) : xa_fwd_dim<_Float16>(A, stream);
+  if (e) return e;
+  RIED_CHECK_LAUNCH("ried_xattn_fwd");
+  return RIED_OK;
+}

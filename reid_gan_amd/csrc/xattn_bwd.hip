@@ -1,0 +1,452 @@
+// Cross attention, backward:  P = exp(S - lse), Dl = sum_c dO o, dP = dO v^T, dS = P (dP - Dl),
+//   dq = scale dS k,  dk = scale dS^T q,  dv = P^T dO.
+// Two kernels, each of which owns what it adds up: rows (dq, over the keys) and keys (dk, dv, over the rows of all heads
+// that share them).  The scores are formed twice - 14 D operations a pair instead of 10 D - and in exchange nothing is
+// added with atomics: the order of every sum is fixed.
+#include "xattn.h"
+
+// fp16 products hold dS only between 2^-24 and 2^16 while P alone spans more: dS travels times a power of two, lowered
+// (and the sums with it) when a value would pass 2^15.  bf16 has fp32's range and needs none.
+template <typename T> struct XaRange {
+  static constexpr bool on = false;
+  static constexpr float p_up = 0.f, p_down = 1.f;               // P times 2^p_up; the sums of P times p_down
+};
+template <> struct XaRange<_Float16> {
+  static constexpr bool on = true;
+  static constexpr float p_up = 15.f, p_down = 0x1p-15f;
+};
+template <int DT>
+__device__ __forceinline__ void xa_fit(float mx, float& es, f32x16 (&acc)[DT]) {
+  if (!__any(mx * es > 32768.f)) return;
+  mx = wave_max(mx);
+  if (!(mx < INFINITY)) return;
+  const float ne = __builtin_amdgcn_exp2f(14.f - ceilf(__log2f(mx))), f = ne / es;
+  if (!(ne < es)) return;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] *= f;
+  es = ne;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// dq: the forward kernel's tiling.  S^T = K Q^T and dP^T = V dO^T per 32 keys, dS^T is the B operand of dq^T += K^T dS^T.
+// Also leaves the rows' exponent base (lse in powers of two, +infinity for a row without keys) and Dl for the other kernel.
+// ---------------------------------------------------------------------------------------------------------------------
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
+  constexpr int KS = XaTile<DP>::KS, DT = XaTile<DP>::DT, RB = XaTile<DP>::RB, NC = XaTile<DP>::NC, RPI = XaTile<DP>::RPI;
+  constexpr int TILE = 64 * RB, NI = 16 / RPI;
+  extern __shared__ __align__(16) char smem[];                    // [2][K tile, V tile]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  int inner, head;
+  xa_block(A.tiles * A.nsplit, A.B * A.Hkv, inner, head);
+  const int b = head / A.Hkv, hk = head % A.Hkv, tile = inner % A.tiles, split = inner / A.tiles;
+  const int row = tile * 128 + wave * 32 + (lane & 31);
+  const bool live = row < A.rows;
+  const int g = live ? row / A.Lq : 0, qi = live ? row - g * A.Lq : 0, hq = hk * A.G + g;
+  const long long flat = (long long)head * A.rows + row;
+  const T* qp = (const T*)A.q + (long long)b * A.qs[0] + (long long)qi * A.qs[1] + (long long)hq * A.qs[2];
+  const T* gp = (const T*)A.dout + (long long)b * A.gs[0] + (long long)qi * A.gs[1] + (long long)hq * A.gs[2];
+  const T* op = (const T*)A.o + (long long)b * A.os[0] + (long long)qi * A.os[1] + (long long)hq * A.os[2];
+  u32x4 fq[KS], fg[KS];
+  float delta = 0.f;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d = s * 16 + h * 8;
+    const bool ok = live && d < A.D;
+    const u32x4 none = {0, 0, 0, 0};
+    fq[s] = ok ? *reinterpret_cast<const u32x4*>(qp + d) : none;
+    fg[s] = ok ? *reinterpret_cast<const u32x4*>(gp + d) : none;
+    const u32x4 fo = ok ? *reinterpret_cast<const u32x4*>(op + d) : none;
+    float x[8], y[8];
+    xa_unpack<T>(fg[s], x);
+    xa_unpack<T>(fo, y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) delta += x[i] * y[i];
+  }
+  {
+    float lo, hi;
+    xa_halves(delta, lo, hi);
+    delta = lo + hi;
+  }
+  float lse2 = INFINITY;
+  if (live) {
+    const float l = A.lse[flat];
+    lse2 = l == -INFINITY ? INFINITY : l * XA_LOG2E;
+    if (split == 0 && h == 0) {
+      A.lse2[flat] = lse2;
+      A.delta[flat] = delta;
+    }
+  }
+  const int nk = xa_keys(A, b), ntile = (nk + 63) >> 6, per = (ntile + A.nsplit - 1) / A.nsplit;
+  const int t0 = split * per, t1 = t0 + per < ntile ? t0 + per : ntile;
+  const char* kp = (const char*)((const T*)A.k + (long long)b * A.ks[0] + (long long)hk * A.ks[2]);
+  const char* vp = (const char*)((const T*)A.v + (long long)b * A.vs[0] + (long long)hk * A.vs[2]);
+  const unsigned char* mp = A.mask ? A.mask + (long long)b * A.ms : nullptr;
+  const int krow = (int)A.ks[1] * 2, vrow = (int)A.vs[1] * 2;
+  const int srow = wave * RPI + lane / NC, sc = (lane % NC) ^ xa_swz(srow);
+  const unsigned dead = sc * 8 >= A.D ? XA_OOB : 0u;
+  const unsigned koff = (unsigned)(srow * krow + sc * 16) | dead, voff = (unsigned)(srow * vrow + sc * 16) | dead;
+  auto issue = [&](int t, u64 w, int buf) {
+    const __amdgpu_buffer_rsrc_t rk = xa_rsrc(kp + (long long)t * 64 * krow), rv = xa_rsrc(vp + (long long)t * 64 * vrow);
+    char* dst = smem + buf * 2 * TILE + wave * RPI * RB;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const unsigned bad = (w >> (srow + i * 4 * RPI)) & 1 ? 0u : XA_OOB;
+      xa_dma16(rk, koff | bad, i * 4 * RPI * krow, dst + i * 4 * RPI * RB);
+      xa_dma16(rv, voff | bad, i * 4 * RPI * vrow, dst + TILE + i * 4 * RPI * RB);
+    }
+  };
+  auto mask_byte = [&](int t) -> int {
+    const int key = t * 64 + lane;
+    return mp && key < nk ? mp[key] : 0;
+  };
+  const float c = A.scale * XA_LOG2E;
+  float es = XaRange<T>::on ? 0x1p24f : 1.f;
+  f32x16 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = xa_zero();
+  u64 w = 0;
+  int byte = 0, buf = 0;
+  if (t0 < t1) {
+    w = xa_word(nk - t0 * 64, mp != nullptr, mask_byte(t0));
+    issue(t0, w, 0);
+    byte = mask_byte(t0 + 1);
+  }
+  for (int t = t0; t < t1; ++t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    u64 wn = 0;
+    if (t + 1 < t1) {
+      wn = xa_word(nk - (t + 1) * 64, mp != nullptr, byte);
+      issue(t + 1, wn, buf ^ 1);
+      byte = mask_byte(t + 2);
+    }
+    if (w) {
+      const char* kt = smem + buf * 2 * TILE;
+      const char* vt = kt + TILE;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f32x16 s = xa_zero(), dp = xa_zero();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          s = xa_mma<T>(xa_frag<DP>(kt, 32 * u, ks, lane), fq[ks], s);
+          dp = xa_mma<T>(xa_frag<DP>(vt, 32 * u, ks, lane), fg[ks], dp);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = xa_exp2(__builtin_fmaf(s[r], c, -lse2));
+        if (w != ~0ull) {                                         // (a hidden key's score reads as 0, not as nothing)
+          const unsigned bits = (unsigned)(w >> (32 * u)) >> (4 * h);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = (bits >> (8 * (r >> 2) + (r & 3))) & 1 ? s[r] : 0.f;
+        }
+        float mx = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[r] *= dp[r] - delta;
+          if constexpr (XaRange<T>::on) mx = fmaxf(mx, fabsf(s[r]));
+        }
+        if constexpr (XaRange<T>::on) {
+          xa_fit<DT>(mx, es, acc);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] *= es;
+        }
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const u32x4 f = xa_as_b<T>(s, kb);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(xa_tr_frag<DP>(kt, u * 32 + kb * 16, d, lane), f, acc[d]);
+        }
+      }
+    }
+    w = wn;
+    buf ^= 1;
+  }
+  if (!live) return;
+  const float f = A.scale / es;
+  if (A.nsplit == 1) {
+    T* dst = (T*)A.dq + (long long)b * A.dqs[0] + (long long)qi * A.dqs[1] + (long long)hq * A.dqs[2];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int ch = d * 32 + 2 * r + 4 * h;
+        if (ch < A.D)
+          *reinterpret_cast<u32x2*>(dst + ch) = u32x2{xa_pack<T>(acc[d][r] * f, acc[d][r + 1] * f),
+                                                      xa_pack<T>(acc[d][r + 2] * f, acc[d][r + 3] * f)};
+      }
+  } else {
+    float* dst = A.part + ((long long)split * A.B * A.Hkv * A.rows + flat) * A.D;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int ch = d * 32 + 2 * r + 4 * h;
+        if (ch < A.D)
+          *reinterpret_cast<f32x4*>(dst + ch) = f32x4{acc[d][r] * f, acc[d][r + 1] * f, acc[d][r + 2] * f, acc[d][r + 3] * f};
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// dk, dv: a block owns 128 keys, a wave 32 of them (K and V fragments in registers), and walks tiles of 64 rows (Q, dO and
+// the rows' two numbers through LDS DMA, two stages).  S = Q K^T and dP = dO V^T have the row along the registers, so P
+// and dS are the B operands of dv^T += dO^T P and dk^T += Q^T dS as they stand.
+// ---------------------------------------------------------------------------------------------------------------------
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xattn_dkv_kernel(XaArgs A) {
+  constexpr int KS = XaTile<DP>::KS, DT = XaTile<DP>::DT, RB = XaTile<DP>::RB, NC = XaTile<DP>::NC, RPI = XaTile<DP>::RPI;
+  constexpr int TILE = 64 * RB, NI = 16 / RPI, STAGE = 2 * TILE + 512;
+  extern __shared__ __align__(16) char smem[];                    // [2][Q tile, dO tile, 64 lse2, 64 Dl]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  int inner, head;
+  xa_block(A.tiles * A.nsplit, A.B * A.Hkv, inner, head);
+  const int b = head / A.Hkv, hk = head % A.Hkv, tile = inner % A.tiles, split = inner / A.tiles;
+  const int key = tile * 128 + wave * 32 + (lane & 31);
+  const int nk = xa_keys(A, b);
+  const bool counts = key < nk && (!A.mask || A.mask[(long long)b * A.ms + key]);
+  const T* kp = (const T*)A.k + (long long)b * A.ks[0] + (long long)key * A.ks[1] + (long long)hk * A.ks[2];
+  const T* vp = (const T*)A.v + (long long)b * A.vs[0] + (long long)key * A.vs[1] + (long long)hk * A.vs[2];
+  u32x4 fk[KS], fv[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d = s * 16 + h * 8;
+    const bool ok = counts && d < A.D;
+    fk[s] = ok ? *reinterpret_cast<const u32x4*>(kp + d) : u32x4{0, 0, 0, 0};
+    fv[s] = ok ? *reinterpret_cast<const u32x4*>(vp + d) : u32x4{0, 0, 0, 0};
+  }
+  const int ntile = (A.rows + 63) >> 6, per = (ntile + A.nsplit - 1) / A.nsplit;
+  const int t0 = split * per;
+  int t1 = t0 + per < ntile ? t0 + per : ntile;
+  if (tile * 128 >= nk) t1 = t0;                                  // no key here counts: zeros
+  const char* qp = (const char*)((const T*)A.q + (long long)b * A.qs[0] + (long long)hk * A.G * A.qs[2]);
+  const char* gp = (const char*)((const T*)A.dout + (long long)b * A.gs[0] + (long long)hk * A.G * A.gs[2]);
+  const __amdgpu_buffer_rsrc_t rq = xa_rsrc(qp), rg = xa_rsrc(gp);   // (host-checked: the heads of a group stay below 2^31 bytes)
+  const __amdgpu_buffer_rsrc_t rl = xa_rsrc(A.lse2 + (long long)head * A.rows), rd = xa_rsrc(A.delta + (long long)head * A.rows);
+  const int qrow = (int)A.qs[1] * 2, qhead = (int)A.qs[2] * 2, grow = (int)A.gs[1] * 2, ghead = (int)A.gs[2] * 2;
+  const int srow = wave * RPI + lane / NC, sc = (lane % NC) ^ xa_swz(srow);
+  const unsigned dead = sc * 8 >= A.D ? XA_OOB : 0u;
+  const float inv_lq = 1.f / (float)A.Lq;
+  auto issue = [&](int t, int buf) {
+    char* st = smem + buf * STAGE;
+    char* dst = st + wave * RPI * RB;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = t * 64 + srow + i * 4 * RPI;
+      int qi;
+      const int g = fast_div(r, A.Lq, inv_lq, qi);
+      const unsigned bad = (r < A.rows ? 0u : XA_OOB) | dead;
+      xa_dma16(rq, (unsigned)(qi * qrow + g * qhead + sc * 16) | bad, 0, dst + i * 4 * RPI * RB);
+      xa_dma16(rg, (unsigned)(qi * grow + g * ghead + sc * 16) | bad, 0, dst + TILE + i * 4 * RPI * RB);
+    }
+    const int r = t * 64 + lane;
+    const unsigned off = r < A.rows ? (unsigned)r * 4u : XA_OOB;
+    if (wave == 0) xa_dma4(rl, off, st + 2 * TILE);
+    if (wave == 1) xa_dma4(rd, off, st + 2 * TILE + 256);
+  };
+  const float c = A.scale * XA_LOG2E;
+  const float up = counts ? XaRange<T>::p_up : -INFINITY;         // (a hidden key's column stays out of the range below)
+  float es = XaRange<T>::on ? 0x1p9f : 1.f;                       // (times the 2^15 of P)
+  f32x16 dv[DT], dk[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) dv[d] = dk[d] = xa_zero();
+  int buf = 0;
+  if (t0 < t1) issue(t0, 0);
+  for (int t = t0; t < t1; ++t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (t + 1 < t1) issue(t + 1, buf ^ 1);
+    const char* qt = smem + buf * STAGE;
+    const char* gt = qt + TILE;
+    const float* rowv = reinterpret_cast<const float*>(qt + 2 * TILE);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f32x16 s = xa_zero(), dp = xa_zero();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        s = xa_mma<T>(xa_frag<DP>(qt, 32 * u, ks, lane), fk[ks], s);
+        dp = xa_mma<T>(xa_frag<DP>(gt, 32 * u, ks, lane), fv[ks], dp);
+      }
+      float mx = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(rowv + 32 * u + 8 * q + 4 * h);
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(rowv + 64 + 32 * u + 8 * q + 4 * h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * q + i;
+          s[r] = xa_exp2(__builtin_fmaf(s[r], c, up - l4[i]));
+          dp[r] = s[r] * (dp[r] - d4[i]);
+          if constexpr (XaRange<T>::on) mx = fmaxf(mx, fabsf(dp[r]));
+        }
+      }
+      if constexpr (XaRange<T>::on) {
+        xa_fit<DT>(mx, es, dk);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] *= es;
+      }
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const u32x4 fp = xa_as_b<T>(s, kb), fs = xa_as_b<T>(dp, kb);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          dv[d] = xa_mma<T>(xa_tr_frag<DP>(gt, u * 32 + kb * 16, d, lane), fp, dv[d]);
+          dk[d] = xa_mma<T>(xa_tr_frag<DP>(qt, u * 32 + kb * 16, d, lane), fs, dk[d]);
+        }
+      }
+    }
+    buf ^= 1;
+  }
+  if (key >= A.Lk) return;
+  // (a hidden key's column was computed from zeros and is dropped, whatever it holds)
+  const float fk_ = A.scale * XaRange<T>::p_down / es, fv_ = XaRange<T>::p_down;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      dk[d][r] = counts ? dk[d][r] * fk_ : 0.f;
+      dv[d][r] = counts ? dv[d][r] * fv_ : 0.f;
+    }
+  if (A.nsplit == 1) {
+    T* pk = (T*)A.dk + (long long)b * A.dks[0] + (long long)key * A.dks[1] + (long long)hk * A.dks[2];
+    T* pv = (T*)A.dv + (long long)b * A.dvs[0] + (long long)key * A.dvs[1] + (long long)hk * A.dvs[2];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int ch = d * 32 + 2 * r + 4 * h;
+        if (ch < A.D) {
+          *reinterpret_cast<u32x2*>(pk + ch) = u32x2{xa_pack<T>(dk[d][r], dk[d][r + 1]), xa_pack<T>(dk[d][r + 2], dk[d][r + 3])};
+          *reinterpret_cast<u32x2*>(pv + ch) = u32x2{xa_pack<T>(dv[d][r], dv[d][r + 1]), xa_pack<T>(dv[d][r + 2], dv[d][r + 3])};
+        }
+      }
+  } else {
+    const long long all = (long long)A.B * A.Hkv * A.Lk, at = (long long)split * all + (long long)head * A.Lk + key;
+    float* pk = A.part + at * A.D;
+    float* pv = pk + A.nsplit * all * A.D;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int ch = d * 32 + 2 * r + 4 * h;
+        if (ch < A.D) {
+          *reinterpret_cast<f32x4*>(pk + ch) = f32x4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
+          *reinterpret_cast<f32x4*>(pv + ch) = f32x4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+        }
+      }
+  }
+}
+
+// adds the shares up: out[b][l][head in group][d] over rows = G * L of each of the B * Hkv heads, 8 channels per thread
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_sum_kernel(const float* __restrict__ part, int nsplit, int heads, int Hkv, int G,
+                                                        int L, int D, T* __restrict__ out, long long sb, long long sl,
+                                                        long long sh) {
+  const int chunks = D >> 3, rows = G * L;
+  const long long all = (long long)heads * rows, i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= all * chunks) return;
+  const long long flat = i / chunks;
+  const int d = (int)(i - flat * chunks) * 8;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f}, e = a;
+  for (int s = 0; s < nsplit; ++s) {
+    const float* p = part + (s * all + flat) * D + d;
+    a += *reinterpret_cast<const f32x4*>(p);
+    e += *reinterpret_cast<const f32x4*>(p + 4);
+  }
+  const int head = (int)(flat / rows), row = (int)(flat - (long long)head * rows);
+  const int b = head / Hkv, hk = head % Hkv, g = row / L, l = row - g * L;
+  *reinterpret_cast<u32x4*>(out + b * sb + l * sl + (long long)(hk * G + g) * sh + d) =
+      u32x4{xa_pack<T>(a[0], a[1]), xa_pack<T>(a[2], a[3]), xa_pack<T>(e[0], e[1]), xa_pack<T>(e[2], e[3])};
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------------
+struct XaBwdPlan { int qtiles, qsplit, ktiles, ksplit; long long rows_all, keys_all, floats; };
+static XaBwdPlan xa_bwd_plan(const ried_xattn_t& d) {
+  const long long rows = d.heads / d.groups * d.queries, heads = d.batch * d.groups;
+  XaBwdPlan p;
+  p.rows_all = heads * rows;
+  p.keys_all = heads * d.keys;
+  auto split = [](long long blocks, long long want, long long most) {
+    long long n = want / (blocks > 0 ? blocks : 1);
+    if (n > most) n = most;
+    if (n > 32) n = 32;
+    return (int)(n < 1 ? 1 : n);
+  };
+  p.qtiles = ceil_div(rows, 128);
+  p.qsplit = split(p.qtiles * heads, 512, d.keys / 256);
+  p.ktiles = ceil_div(d.keys, 128);
+  p.ksplit = split(p.ktiles * heads, d.dim <= 64 ? 512 : 256, rows / 256);
+  const long long a = p.qsplit > 1 ? p.qsplit * p.rows_all * d.dim : 0, b = p.ksplit > 1 ? 2 * p.ksplit * p.keys_all * d.dim : 0;
+  p.floats = 2 * ((p.rows_all + 3) / 4 * 4) + (a > b ? a : b);
+  return p;
+}
+
+extern "C" long long ried_xattn_bwd_scratch_floats(long long batch, long long queries, long long keys, int heads,
+                                                   int groups, int dim) {
+  if (batch <= 0 || queries <= 0 || heads <= 0 || groups <= 0 || heads % groups) return 0;
+  ried_xattn_t d = {};
+  d.batch = batch; d.queries = queries; d.keys = keys; d.heads = heads; d.groups = groups; d.dim = dim;
+  return xa_bwd_plan(d).floats;
+}
+
+template <typename T, int DP>
+static int xa_bwd_launch(XaArgs A, const XaBwdPlan& p, hipStream_t stream) {
+  constexpr int lq = 2 * 2 * 64 * XaTile<DP>::RB, lk = lq + 2 * 512;
+  for (int i = 0; i < 2; ++i) {
+    const hipError_t e = hipFuncSetAttribute(i ? (const void*)xattn_dkv_kernel<T, DP> : (const void*)xattn_dq_kernel<T, DP>,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, i ? lk : lq);
+    RIED_CHECK_ARG(e == hipSuccess, "ried_xattn_bwd: LDS: %s", hipGetErrorString(e));
+  }
+  const int heads = A.B * A.Hkv;
+  A.tiles = p.qtiles;
+  A.nsplit = p.qsplit;
+  hipLaunchKernelGGL((xattn_dq_kernel<T, DP>), dim3((unsigned)(A.tiles * A.nsplit * heads)), dim3(256), lq, stream, A);
+  if (A.nsplit > 1)
+    hipLaunchKernelGGL((xattn_sum_kernel<T>), dim3(ceil_div(p.rows_all * (A.D >> 3), 256)), dim3(256), 0, stream, A.part,
+                       A.nsplit, heads, A.Hkv, A.G, A.Lq, A.D, (T*)A.dq, A.dqs[0], A.dqs[1], A.dqs[2]);
+  if (A.Lk == 0) return RIED_OK;
+  A.tiles = p.ktiles;
+  A.nsplit = p.ksplit;
+  hipLaunchKernelGGL((xattn_dkv_kernel<T, DP>), dim3((unsigned)(A.tiles * A.nsplit * heads)), dim3(256), lk, stream, A);
+  if (A.nsplit > 1) {
+    hipLaunchKernelGGL((xattn_sum_kernel<T>), dim3(ceil_div(p.keys_all * (A.D >> 3), 256)), dim3(256), 0, stream, A.part,
+                       A.nsplit, heads, A.Hkv, 1, A.Lk, A.D, (T*)A.dk, A.dks[0], A.dks[1], A.dks[2]);
+    hipLaunchKernelGGL((xattn_sum_kernel<T>), dim3(ceil_div(p.keys_all * (A.D >> 3), 256)), dim3(256), 0, stream,
+                       A.part + A.nsplit * p.keys_all * A.D, A.nsplit, heads, A.Hkv, 1, A.Lk, A.D, (T*)A.dv, A.dvs[0],
+                       A.dvs[1], A.dvs[2]);
+  }
+  return RIED_OK;
+}
+template <typename T>
+static int xa_bwd_dim(const XaArgs& A, const XaBwdPlan& p, hipStream_t stream) {
+  return A.D <= 32 ? xa_bwd_launch<T, 32>(A, p, stream) : A.D <= 64 ? xa_bwd_launch<T, 64>(A, p, stream)
+       : A.D <= 96 ? xa_bwd_launch<T, 96>(A, p, stream) : xa_bwd_launch<T, 128>(A, p, stream);
+}
+
+extern "C" int ried_xattn_bwd(const ried_xattn_t* desc, hipStream_t stream) {
+  if (int e = xa_check(desc, "ried_xattn_bwd", true)) return e;
+  const ried_xattn_t& d = *desc;
+  if (d.batch == 0) return RIED_OK;
+  RIED_CHECK_ARG(d.queries > 0, "ried_xattn_bwd: no queries (dk and dv are zeros: fill them)");
+  RIED_CHECK_ARG(d.lse && d.scratch, "ried_xattn_bwd: lse and ried_xattn_bwd_scratch_floats() of scratch are needed");
+  const long long G = d.heads / d.groups;
+  RIED_CHECK_ARG(G * d.queries < (1ll << 29), "ried_xattn_bwd: sizes out of range");
+  for (const long long* s : {d.q_stride, d.dout_stride})
+    RIED_CHECK_ARG((d.queries * s[1] + G * s[2]) * 2 < (1ll << 31),
+                   "ried_xattn_bwd: the heads of a group span over 2^31 bytes of q or dout: pass fewer queries");
+  XaArgs A = xa_args(d);
+  const XaBwdPlan p = xa_bwd_plan(d);
+  RIED_CHECK_ARG((long long)p.qtiles * p.qsplit * A.B * A.Hkv <= 0x7fffffffll && (long long)p.ktiles * p.ksplit * A.B * A.Hkv <= 0x7fffffffll,
+                 "ried_xattn_bwd: too many blocks");
+  const long long pad = (p.rows_all + 3) / 4 * 4;
+  A.lse2 = d.scratch;
+  A.delta = d.scratch + pad;
+  A.part = d.scratch + 2 * pad;
+  const int e = d.type == RIED_T_BF16 ? xa_bwd_dim<bf16_t>(A, p, stream) : xa_bwd_dim<_Float16>(A, p, stream);
+  if (e) return e;
+  RIED_CHECK_LAUNCH("ried_xattn_bwd");
+  return RIED_OK;
+}

@@ -5,7 +5,10 @@ computation below is a hand-written HIP kernel in libried_gan.so.
 """
 from __future__ import annotations
 
+import contextlib
+import struct
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -13,6 +16,7 @@ import torch
 from ._lib import lib
 
 BF16 = torch.bfloat16
+_HERE = contextlib.nullcontext()
 
 
 def _stream() -> int:
@@ -732,3 +736,96 @@ def ssim_fwd(a, b, ref, c1, c2, sums, gmap=None, clamp=None):
 def ssim_bwd(a, ref, gmap, scale, da, scale_dev=None, accumulate=False):
     n, h, w = ref.shape[0], ref.shape[-2], ref.shape[-1]
     lib.ried_ssim_bwd(_p(a), _p(ref), _p(gmap), n, h, w, scale, _p(scale_dev), _p(da), int(accumulate), _stream())
+
+
+# --------------------------------------------------------------------------- token operators
+# Layer norm, rotary positions, cross attention and AdamW over many tensors.  These run on the device of their first
+# tensor, whatever the current one is, on that device's current stream.
+TOKEN_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_XATTN = struct.Struct("=12q24q8qd")           # ried_xattn_t
+
+
+def on_device(t: torch.Tensor):
+    """Context in which `t`'s device is the current one."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def layer_norm_fwd(x: torch.Tensor, w, b, y: torch.Tensor, mean, rstd, eps: float):
+    """y = (x - mean) * rstd * w + b over the rows of x [rows][C] (row strides x.stride(0), y.stride(0)); w, b may be
+    None; mean, rstd: fp32 [rows] or None."""
+    with on_device(x):
+        lib.ried_layer_norm_fwd(x.data_ptr(), x.stride(0), _p(w), _p(b), y.data_ptr(), y.stride(0), _p(mean), _p(rstd),
+                                x.shape[0], x.shape[1], eps, TOKEN_TYPES[x.dtype], 0 if w is None else TOKEN_TYPES[w.dtype],
+                                _stream())
+
+
+def layer_norm_bwd_scratch_floats(rows: int, C: int, dtype: torch.dtype) -> int:
+    return lib.ried_layer_norm_bwd_scratch_floats(rows, C, TOKEN_TYPES[dtype])
+
+
+def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, w, mean, rstd, dx: torch.Tensor, dw, db, scratch):
+    """dx, and the parameter gradients dw = sum dy * xh, db = sum dy (None: not wanted) of layer_norm_fwd."""
+    wt = w if w is not None else dw if dw is not None else db
+    with on_device(x):
+        lib.ried_layer_norm_bwd(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), _p(w), mean.data_ptr(),
+                                rstd.data_ptr(), dx.data_ptr(), dx.stride(0), _p(dw), _p(db), _p(scratch), x.shape[0],
+                                x.shape[1], TOKEN_TYPES[x.dtype], 0 if wt is None else TOKEN_TYPES[wt.dtype], _stream())
+
+
+def rotary(x: torch.Tensor, y: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sections, interleaved: bool,
+           inverse: bool):
+    """y = x [B][L][H][D] turned by its positions [B][L][axes]; y may be x."""
+    B, L, H, D = x.shape
+    s = tuple(sections) + (0,) * (4 - len(sections))
+    xs, ys, ps = x.stride(), y.stride(), positions.stride()
+    with on_device(x):
+        lib.ried_rotary(x.data_ptr(), xs[0], xs[1], xs[2], y.data_ptr(), ys[0], ys[1], ys[2], positions.data_ptr(),
+                        POSITION_TYPES[positions.dtype], ps[0], ps[1], ps[2], freqs.data_ptr(), s[0], s[1], s[2], s[3],
+                        B, L, H, D, interleaved, inverse, TOKEN_TYPES[x.dtype], _stream())
+
+
+def _xattn_desc(q, k, v, o, lse, lengths, key_mask, scratch, scale, dout=None, dq=None, dk=None, dv=None) -> bytes:
+    B, Lq, H, D = q.shape
+    zero = (0, 0, 0)
+    back = dout is not None
+    return _XATTN.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        0 if lengths is None else lengths.data_ptr(), 0 if key_mask is None else key_mask.data_ptr(),
+        0 if scratch is None else scratch.data_ptr(), *((t.data_ptr() for t in (dout, dq, dk, dv)) if back else (0, 0, 0, 0)),
+        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3],
+        *(dout.stride()[:3] if back else zero), *(dq.stride()[:3] if back else zero), *(dk.stride()[:3] if back else zero),
+        *(dv.stride()[:3] if back else zero), 0 if key_mask is None else key_mask.stride(0), B, Lq, k.shape[1], H, k.shape[2],
+        D, TOKEN_TYPES[q.dtype], scale)
+
+
+@lru_cache(maxsize=4096)
+def xattn_fwd_scratch_floats(batch: int, queries: int, keys: int, heads: int, groups: int, dim: int) -> int:
+    return lib.ried_xattn_fwd_scratch_floats(batch, queries, keys, heads, groups, dim)
+
+
+@lru_cache(maxsize=4096)
+def xattn_bwd_scratch_floats(batch: int, queries: int, keys: int, heads: int, groups: int, dim: int) -> int:
+    return lib.ried_xattn_bwd_scratch_floats(batch, queries, keys, heads, groups, dim)
+
+
+def xattn_fwd(q, k, v, out, lse, scale: float, lengths=None, key_mask=None, scratch=None):
+    """out [B][queries][heads][D] = attention of q over k, v [B][keys][key heads][D]; lse fp32 [B][heads][queries] or
+    None; lengths int32 [B], key_mask one byte per [B][keys]; scratch: xattn_fwd_scratch_floats() floats."""
+    with on_device(q):
+        lib.ried_xattn_fwd(_xattn_desc(q, k, v, out, lse, lengths, key_mask, scratch, scale), _stream())
+
+
+def xattn_bwd(dout, q, k, v, out, lse, dq, dk, dv, scale: float, scratch, lengths=None, key_mask=None):
+    """dq, dk, dv (all written) of xattn_fwd; scratch: xattn_bwd_scratch_floats() floats."""
+    with on_device(q):
+        lib.ried_xattn_bwd(_xattn_desc(q, k, v, out, lse, lengths, key_mask, scratch, scale, dout, dq, dk, dv), _stream())
+
+
+def adamw_jobs(jobs, blockmap, grads, first, steps, coef, lr, b1, b2, eps, weight_decay, dtype: torch.dtype, state_bits: int):
+    """One AdamW step over the tensors of a job table (reid_gan_amd.optim builds it).  grads, first: host arrays
+    (array('q') of addresses, array('i'))."""
+    with on_device(jobs):
+        lib.ried_adamw_jobs(jobs.data_ptr(), blockmap.data_ptr(), grads.buffer_info()[0], first.buffer_info()[0], len(grads),
+                            steps.data_ptr(), coef.data_ptr(), lr, b1, b2, eps, weight_decay, TOKEN_TYPES[dtype], state_bits,
+                            _stream())

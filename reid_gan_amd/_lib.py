@@ -97,9 +97,22 @@ class _Lib:
             raise RuntimeError(f"{name} failed ({rc}): {msg.decode() if msg else '?'}")
 
     def __getattr__(self, name):
-        if name.startswith("ried_"):
-            return lambda *a: self.call(name, *a)
-        raise AttributeError(name)
+        """First use of an entry point: bind it as an attribute, so that later calls go straight to it (the look-up by name
+        costs a small kernel's launch again)."""
+        if not name.startswith("ried_"):
+            raise AttributeError(name)
+        dll = self.load()
+        fn = getattr(dll, name)
+        if not name.endswith(_VALUE_SUFFIXES):
+            entry = fn
+
+            def fn(*args):
+                rc = entry(*args)
+                if rc != 0:
+                    msg = dll.ried_last_error()
+                    raise RuntimeError(f"{name} failed ({rc}): {msg.decode() if msg else '?'}")
+        self.__dict__[name] = fn
+        return fn
 
 
 lib = _Lib()

@@ -13,7 +13,6 @@ gradients the functions here may be captured as they are.
 """
 from __future__ import annotations
 
-import math
 from typing import Optional, Sequence
 
 import torch
@@ -24,19 +23,21 @@ from . import ops
 __all__ = ["layer_norm", "LayerNorm", "rotary", "rotary_frequencies", "cross_attention"]
 
 F32 = torch.float32
+_CONTIGUOUS = torch.contiguous_format
+_CROSS_TYPES = (torch.bfloat16, torch.float16)
 
 
 def _check_tensor(what: str, name: str, t, types, device=None):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: {name} is a tensor, not {type(t).__name__}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{what}: {name} is on {t.device}, not on {device}")
     if t.dtype not in types:
         raise TypeError(f"{what}: {name} is {t.dtype}, not one of {', '.join(str(d).replace('torch.', '') for d in types)}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{what}: {name} is on {t.device}, not on {device}")
 
 
 def _on_gpu(what: str, t: torch.Tensor):
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"{what}: tensors must be on a ROCm device; there is no CPU path")
 
 
@@ -46,20 +47,25 @@ def _not_captured(what: str):
                            "functions of reid_gan_amd.ops instead")
 
 
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _once(backward):
+    """A backward function without a second derivative: asking for one raises.  (once_differentiable says so too, at the
+    price of a small kernel's launch in every first derivative.)"""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, grad):
+        return guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
+    return run
 
 
 # --------------------------------------------------------------------------- layer norm
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t as [rows][C] with adjacent channels and rows that do not overlap (a copy only where no such view exists)."""
+    """t, or a view (a copy where there is none) as [rows][C], with adjacent channels and rows that do not overlap."""
+    if t.is_contiguous():
+        return t
     C = t.shape[-1]
-    if t.dim() != 2:
-        t = t.reshape(-1, C) if t.dim() > 1 else t.unsqueeze(0)
-    if (C > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < C):
+    t = t.reshape(-1, C)
+    if (C > 1 and t.stride(1) != 1) or t.stride(0) < C:
         t = t.contiguous()
-    if t.stride(0) < C or (C == 1 and t.stride(1) != 1):
-        t = t.as_strided(t.shape, (max(C, t.stride(0)), 1))      # one row, or one channel: strides that nothing uses
     return t
 
 
@@ -68,36 +74,32 @@ class _LayerNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps):
         _not_captured("layer_norm")
         rows = _rows(x)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        mean, rstd = torch.empty(2, rows.shape[0], dtype=F32, device=x.device)
-        ops.layer_norm_fwd(rows, weight, bias, y.view(rows.shape), mean, rstd, eps)
-        ctx.save_for_backward(rows, weight, mean, rstd)
-        ctx.shape, ctx.bias_type = x.shape, None if bias is None else bias.dtype
+        y = torch.empty_like(x, memory_format=_CONTIGUOUS)
+        stats = x.new_empty((2, x.numel() // x.shape[-1]), dtype=F32)
+        ops.layer_norm_fwd(rows, weight, bias, y, stats, eps)
+        ctx.save_for_backward(rows, weight, stats)
+        ctx.meta = x.shape, None if bias is None else bias.dtype
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         _not_captured("layer_norm")
-        rows, weight, mean, rstd = ctx.saved_tensors
-        n, C = rows.shape
-        dx = torch.empty(n, C, dtype=rows.dtype, device=rows.device)
-        dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
-        db = torch.empty(C, dtype=ctx.bias_type, device=rows.device) if ctx.needs_input_grad[2] else None
+        rows, weight, stats = ctx.saved_tensors
+        shape, bias_type = ctx.meta
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        C = shape[-1]
+        dx = torch.empty_like(rows, memory_format=_CONTIGUOUS)
+        dw = torch.empty_like(weight) if need_w else None
+        db = rows.new_empty((C,), dtype=bias_type) if need_b else None
         scratch = None
-        if dw is not None or db is not None:
-            scratch = torch.empty(ops.layer_norm_bwd_scratch_floats(n, C, rows.dtype), dtype=F32, device=rows.device)
-        ops.layer_norm_bwd(_rows(dy), rows, weight, mean, rstd, dx, dw, db, scratch)
-        return dx.view(ctx.shape) if ctx.needs_input_grad[0] else None, dw, db, None
+        if need_w or need_b:
+            scratch = stats.new_empty((ops.layer_norm_bwd_scratch_floats(stats.shape[1], C, rows.dtype),))
+        ops.layer_norm_bwd(_rows(dy), rows, weight, stats, dx, dw, db, scratch)
+        return dx.view(shape) if need_x else None, dw, db, None
 
 
-def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
-               eps: float = 1e-5) -> torch.Tensor:
-    """Layer norm over the last axis: (x - mean) / sqrt(var + eps) * weight + bias.
-
-    x: any shape; rows are read where they lie when their channels are adjacent.  weight, bias: [C], contiguous, both fp32
-    or both of x's type, each optional.  The result is contiguous and of x's type; weight and bias gradients are summed
-    in fp32 in a fixed order."""
+def _check_layer_norm(x, weight, bias, eps):
     _check_tensor("layer_norm", "x", x, ops.TOKEN_TYPES)
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("layer_norm: x has no last axis to normalise")
@@ -112,11 +114,21 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if not eps >= 0:
         raise ValueError("layer_norm: eps is negative")
     _on_gpu("layer_norm", x)
-    if _wants_grad(x, weight, bias):
-        return _LayerNormFn.apply(x, weight, bias, float(eps))
-    rows = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    ops.layer_norm_fwd(rows, weight, bias, y if y.dim() == 2 else y.view(rows.shape), None, None, float(eps))
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the last axis: (x - mean) / sqrt(var + eps) * weight + bias.
+
+    x: any shape; rows are read where they lie when their channels are adjacent.  weight, bias: [C], contiguous, both fp32
+    or both of x's type, each optional.  The result is contiguous and of x's type; weight and bias gradients are summed
+    in fp32 in a fixed order."""
+    _check_layer_norm(x, weight, bias, eps)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        return _LayerNormFn.apply(x, weight, bias, eps)
+    y = torch.empty_like(x, memory_format=_CONTIGUOUS)
+    ops.layer_norm_fwd(_rows(x), weight, bias, y, None, eps)
     return y
 
 
@@ -160,19 +172,19 @@ class _RotaryFn(torch.autograd.Function):
         _not_captured("rotary")
         ctx.save_for_backward(positions, freqs)
         ctx.meta = (sections, interleaved, inverse)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = torch.empty_like(x, memory_format=_CONTIGUOUS)
         ops.rotary(x, y, positions, freqs, sections, interleaved, inverse)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         _not_captured("rotary")
         positions, freqs = ctx.saved_tensors
         sections, interleaved, inverse = ctx.meta
         if dy.stride(-1) != 1:
             dy = dy.contiguous()
-        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+        dx = torch.empty_like(dy, memory_format=_CONTIGUOUS)
         ops.rotary(dy, dx, positions, freqs, sections, interleaved, not inverse)
         return dx, None, None, None, None, None
 
@@ -189,42 +201,43 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sectio
     _check_tensor("rotary", "x", x, ops.TOKEN_TYPES)
     if x.dim() != 4:
         raise ValueError("rotary: x is [batch][tokens][heads][channels]")
-    sections = tuple(int(n) for n in sections)
-    pairs = sum(sections)
-    if not 1 <= len(sections) <= 4 or min(sections) < 0 or not 0 < 2 * pairs <= x.shape[3]:
-        raise ValueError(f"rotary: sections {sections} do not fit {x.shape[3]} channels (one to four axes, two channels a pair)")
+    B, L, _, D = x.shape
+    axes, pairs = len(sections), sum(sections)
+    if not 1 <= axes <= 4 or min(sections) < 0 or not 0 < 2 * pairs <= D:
+        raise ValueError(f"rotary: sections {tuple(sections)} do not fit {D} channels (one to four axes, two channels a pair)")
     _check_tensor("rotary", "positions", positions, ops.POSITION_TYPES, x.device)
     if positions.dim() == 2:
-        positions = positions.unsqueeze(0).expand(x.shape[0], -1, -1)
-    if positions.shape != (x.shape[0], x.shape[1], len(sections)):
-        raise ValueError(f"rotary: positions are [batch][tokens][{len(sections)}] for x {tuple(x.shape)}, not {tuple(positions.shape)}")
+        positions = positions.unsqueeze(0).expand(B, -1, -1)
+    if positions.shape != (B, L, axes):
+        raise ValueError(f"rotary: positions are [batch][tokens][{axes}] for x {tuple(x.shape)}, not {tuple(positions.shape)}")
     _check_tensor("rotary", "freqs", freqs, (torch.float64,), x.device)
     if freqs.shape != (pairs,) or not freqs.is_contiguous():
         raise ValueError(f"rotary: freqs is a contiguous table of {pairs} entries")
-    if out is x and x.stride(3) != 1 and x.shape[3] > 1:
-        raise ValueError("rotary: in place needs adjacent channels")
+    adjacent = D == 1 or x.stride(3) == 1
     if out is None:
         _on_gpu("rotary", x)
-        if x.stride(3) != 1 and x.shape[3] > 1:
+        if not adjacent:
             x = x.contiguous()
-        if _wants_grad(x):
-            return _RotaryFn.apply(x, positions, freqs, sections, bool(interleaved), bool(inverse))
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        if x.requires_grad and torch.is_grad_enabled():
+            return _RotaryFn.apply(x, positions, freqs, tuple(sections), interleaved, inverse)
+        out = torch.empty_like(x, memory_format=_CONTIGUOUS)
     else:
-        if _wants_grad(x, out):
+        if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
             raise RuntimeError("rotary: out= has no gradient; leave it out, or use torch.no_grad()")
+        if out is x and not adjacent:
+            raise ValueError("rotary: in place needs adjacent channels")
         _check_tensor("rotary", "out", out, (x.dtype,), x.device)
-        if out.shape != x.shape or (out.stride(3) != 1 and out.shape[3] > 1):
+        if out.shape != x.shape or (out.stride(3) != 1 and D > 1):
             raise ValueError("rotary: out has x's shape and adjacent channels")
         if any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride())):
             raise ValueError("rotary: out is an expanded tensor")
         same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
-        if not same and x.numel() and (_overlap(out, x) or _overlap(out, positions)):
-            raise ValueError("rotary: out overlaps x or positions without being x")
+        if x.numel() and ((not same and _overlap(out, x)) or _overlap(out, positions) or _overlap(out, freqs)):
+            raise ValueError("rotary: out overlaps x, positions or freqs without being x")
         _on_gpu("rotary", x)
-        if x.stride(3) != 1 and x.shape[3] > 1:
+        if not adjacent:
             x = x.contiguous()
-    ops.rotary(x, out, positions, freqs, sections, bool(interleaved), bool(inverse))
+    ops.rotary(x, out, positions, freqs, sections, interleaved, inverse)
     return out
 
 
@@ -232,17 +245,17 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sectio
 def _laid_out(t: torch.Tensor) -> torch.Tensor:
     """t [batch][tokens][heads][channels] as the kernels read it: adjacent channels, strides in multiples of 8 elements,
     16-byte alignment (a copy only where it is not)."""
-    s = t.stride()
-    if s[3] == 1 and not (s[0] | s[1] | s[2]) & 7 and s[0] >= 0 and 0 <= s[1] <= 1 << 23 and s[2] >= 0 and not t.data_ptr() & 15:
+    a, b, c, d = t.stride()
+    if d == 1 and not ((a | b | c) & 7 or t.data_ptr() & 15) and a >= 0 and 0 <= b <= 1 << 23 and c >= 0:
         return t
-    return t.clone(memory_format=torch.contiguous_format)
+    return t.clone(memory_format=_CONTIGUOUS)
 
 
 def _attend(q, k, v, lengths, key_mask, scale, lse):
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    n = ops.xattn_fwd_scratch_floats(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3])
-    scratch = torch.empty(n, dtype=F32, device=q.device) if n else None
-    ops.xattn_fwd(q, k, v, out, lse, scale, lengths, key_mask, scratch)
+    (B, Lq, H, D), (_, Lk, G, _) = q.shape, k.shape
+    out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    n = ops.xattn_fwd_scratch_floats(B, Lq, Lk, H, G, D)
+    ops.xattn_fwd(q, k, v, out, lse, scale, lengths, key_mask, q.new_empty((n,), dtype=F32) if n else None)
     return out
 
 
@@ -251,22 +264,23 @@ class _CrossFn(torch.autograd.Function):
     def forward(ctx, q, k, v, lengths, key_mask, scale):
         _not_captured("cross_attention")
         q, k, v = _laid_out(q), _laid_out(k), _laid_out(v)
-        lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=F32, device=q.device)
+        B, Lq, H, _ = q.shape
+        lse = q.new_empty((B, H, Lq), dtype=F32)
         out = _attend(q, k, v, lengths, key_mask, scale, lse)
         ctx.save_for_backward(q, k, v, out, lse, lengths, key_mask)
         ctx.scale = scale
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         _not_captured("cross_attention")
         q, k, v, out, lse, lengths, key_mask = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        if q.shape[1] == 0:
+        dq, dk, dv = (torch.empty_like(t, memory_format=_CONTIGUOUS) for t in (q, k, v))
+        (B, Lq, H, D), (_, Lk, G, _) = q.shape, k.shape
+        if Lq == 0:
             return dq, dk.zero_(), dv.zero_(), None, None, None
-        n = ops.xattn_bwd_scratch_floats(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3])
-        scratch = torch.empty(n, dtype=F32, device=q.device)
+        scratch = lse.new_empty((ops.xattn_bwd_scratch_floats(B, Lq, Lk, H, G, D),))
         ops.xattn_bwd(_laid_out(dout), q, k, v, out, lse, dq, dk, dv, ctx.scale, scratch, lengths, key_mask)
         return dq, dk, dv, None, None, None
 
@@ -281,32 +295,33 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: 
     keys gives zeros and no gradient; hidden keys have no effect whatever they hold, and get zero gradients.  scale:
     channels ** -0.5 unless given.  channels: a multiple of 8 up to 128, bf16 or fp16.  Views are read where they lie when
     their channels are adjacent and their strides are multiples of 8 elements; others are copied."""
-    types = (torch.bfloat16, torch.float16)
-    _check_tensor("cross_attention", "q", q, types)
-    _check_tensor("cross_attention", "k", k, (q.dtype,), q.device)
-    _check_tensor("cross_attention", "v", v, (q.dtype,), q.device)
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+    _check_tensor("cross_attention", "q", q, _CROSS_TYPES)
+    device, kind = q.device, (q.dtype,)
+    _check_tensor("cross_attention", "k", k, kind, device)
+    _check_tensor("cross_attention", "v", v, kind, device)
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape or qs[0] != ks[0] or qs[3] != ks[3]:
         raise ValueError(f"cross_attention: q [batch][queries][heads][channels] and k, v [batch][keys][key heads][channels] do "
-                         f"not fit: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    B, Lq, H, D = q.shape
-    if H == 0 or k.shape[2] == 0 or H % k.shape[2]:
-        raise ValueError(f"cross_attention: {H} heads do not divide over {k.shape[2]} key heads")
+                         f"not fit: {tuple(qs)}, {tuple(ks)}, {tuple(v.shape)}")
+    B, _, H, D = qs
+    if H == 0 or ks[2] == 0 or H % ks[2]:
+        raise ValueError(f"cross_attention: {H} heads do not divide over {ks[2]} key heads")
     if D % 8 or not 8 <= D <= 128:
         raise ValueError(f"cross_attention: {D} channels are not a multiple of 8 up to 128")
     if lengths is not None:
-        _check_tensor("cross_attention", "lengths", lengths, (torch.int32,), q.device)
+        _check_tensor("cross_attention", "lengths", lengths, (torch.int32,), device)
         if lengths.shape != (B,) or not lengths.is_contiguous():
             raise ValueError(f"cross_attention: lengths is a contiguous [{B}] tensor")
     if key_mask is not None:
-        _check_tensor("cross_attention", "key_mask", key_mask, (torch.bool, torch.uint8), q.device)
+        _check_tensor("cross_attention", "key_mask", key_mask, (torch.bool, torch.uint8), device)
         if key_mask.shape != (B, k.shape[1]):
             raise ValueError(f"cross_attention: key_mask is [{B}][{k.shape[1]}], not {tuple(key_mask.shape)}")
         if key_mask.stride(0) < 0 or (key_mask.stride(1) != 1 and key_mask.shape[1] > 1):
             key_mask = key_mask.contiguous()
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0 < scale < 1e30 or math.isnan(scale):
+    if not 0 < scale < 1e30:
         raise ValueError("cross_attention: scale is a positive number")
     _on_gpu("cross_attention", q)
-    if _wants_grad(q, k, v):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _CrossFn.apply(q, k, v, lengths, key_mask, scale)
     return _attend(_laid_out(q), _laid_out(k), _laid_out(v), lengths, key_mask, scale, None)

@@ -317,7 +317,7 @@ static LnPlan ln_plan(int type, int C) {
   if (chunks <= 256) return {4, 64, 1};
   if (chunks <= 512) return {2, 64, 4};
   if (chunks <= 1024) return {4, 64, 4};
-  if (chunks <= 4096) return {4, 64, 16};
+  if (chunks <= 2048) return {2, 64, 16};                       // (wider in registers would spill at 16 waves)
   return {0, 0, 0};
 }
 #define LN_PLANS(M)                                                                                                  \
@@ -327,9 +327,9 @@ static LnPlan ln_plan(int type, int C) {
   else if (pl.nv == 1) { M(1, 64, 1) }                                                                               \
   else if (pl.nv == 2 && pl.wpr == 1) { M(2, 64, 1) }                                                                \
   else if (pl.wpr == 1) { M(4, 64, 1) }                                                                              \
+  else if (pl.wpr == 16) { M(2, 64, 16) }                                                                            \
   else if (pl.nv == 2) { M(2, 64, 4) }                                                                               \
-  else if (pl.wpr == 4) { M(4, 64, 4) }                                                                              \
-  else { M(4, 64, 16) }
+  else { M(4, 64, 4) }
 
 static int ln_parts(long long rows, int type, int C) {
   const LnPlan pl = ln_plan(type, C);

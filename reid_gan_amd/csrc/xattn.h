@@ -9,10 +9,12 @@
 // matching A operand comes out of LDS through the transposing read with its k rows addressed in that order.
 //
 // An LDS tile holds 64 rows (keys, or query rows) of 128 or 256 bytes; 16-byte chunk c of row r is stored in slot
-// c ^ swz(r), which spreads both the row-wise 16-byte reads (8 rows per cycle) and the transposing 8-byte reads (4 rows
-// by 64 bytes) evenly over the banks.  Tiles are filled by LDS DMA: its destination is lane-linear, so the swizzle is
-// applied to the chunk a lane fetches; rows and chunks that do not exist (past the end, hidden keys, channels past D)
-// use an offset outside the descriptor and arrive as zeros - whatever a hidden key holds never reaches a product.
+// c ^ swz(r).  The LDS serves 256 bytes a cycle: 16 lanes of a row-wise 16-byte read, whose 16 rows put a chunk into 16
+// different places of the 256 bytes, or 32 lanes of a transposing 8-byte read, which takes 64 bytes of 4 rows.  (Measured:
+// 4 and 2 cycles an instruction without conflicts; a swizzle over 8 places cost the former 4 more.)  Tiles are filled by LDS
+// DMA: its destination is lane-linear, so the swizzle is applied to the chunk a lane fetches; rows and chunks that do not
+// exist (past the end, hidden keys, channels past D) use an offset outside the descriptor and arrive as zeros - whatever
+// a hidden key holds never reaches a product.
 #pragma once
 #include "tokens.h"
 #include "../../include/ried_gan.h"
@@ -23,6 +25,7 @@ typedef __attribute__((ext_vector_type(2))) _Float16 pk_f16x2;
 typedef __attribute__((address_space(3))) s16x4 xa_lds_s16x4;
 typedef unsigned long long u64;
 
+template <int N> struct XaInt { static constexpr int value = N; };
 #define XA_OOB 0x80000000u
 #define XA_LOG2E 1.44269504088896340736f
 #define XA_LN2 0.69314718055994530942f
@@ -56,7 +59,9 @@ __device__ __forceinline__ f32x16 xa_zero() {
   return z;
 }
 
-__device__ __forceinline__ int xa_swz(int r) { return ((r & 1) << 2) | ((r >> 1) & 3); }
+template <int RB> __device__ __forceinline__ int xa_swz(int r) {
+  return RB == 256 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+}
 
 // (lo, hi): this lane's value and that of lane ^ 32, in lane order
 __device__ __forceinline__ void xa_halves(float v, float& lo, float& hi) {
@@ -85,20 +90,74 @@ template <int DP> struct XaTile {
 template <int DP>
 __device__ __forceinline__ u32x4 xa_frag(const char* tile, int rowbase, int ks, int lane) {
   constexpr int RB = XaTile<DP>::RB;
-  const int r = lane & 31, c = (2 * ks + (lane >> 5)) ^ xa_swz(r);
+  const int r = lane & 31, c = (2 * ks + (lane >> 5)) ^ xa_swz<RB>(r);
   return *reinterpret_cast<const u32x4*>(tile + (rowbase + r) * RB + c * 16);
 }
-// Fragment of channels 32 dt .. + 31 (the operand's rows), contraction over the 16 tile rows from rowbase (paired order)
-template <int DP>
-__device__ __forceinline__ u32x4 xa_tr_frag(const char* tile, int rowbase, int dt, int lane) {
-  constexpr int RB = XaTile<DP>::RB;
-  const int h = lane >> 5, rg = (lane >> 4) & 1, q = (lane >> 2) & 3, p = lane & 3, k0 = 4 * h + q;
-  const int c = (dt * 4 + rg * 2 + (p >> 1)) ^ xa_swz(k0);
-  const char* a = tile + (rowbase + k0) * RB + c * 16 + (p & 1) * 8;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((xa_lds_s16x4*)a);
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((xa_lds_s16x4*)(a + 8 * RB));
-  const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
-  return u32x4{l2[0], l2[1], h2[0], h2[1]};
+// Fragments of channels 32 dt .. + 31 (the operand's rows) for all dt, contraction over the 16 tile rows from ROW (paired
+// order).  Written in assembly, its wait included: the compiler cannot tell the transposing read from the DMA stage that
+// is being filled and would wait for that first, which puts a memory round trip into every tile.
+template <int DP> struct XaTr {
+  unsigned at[2][XaTile<DP>::DT];                                 // this lane's LDS addresses in the first tile: rows k0, k0 + 8
+  __device__ __forceinline__ XaTr(const char* tile, int lane) {
+    constexpr int RB = XaTile<DP>::RB;
+    const int h = lane >> 5, rg = (lane >> 4) & 1, q = (lane >> 2) & 3, p = lane & 3, k0 = 4 * h + q;
+    static_assert(RB == 256 || XaTile<DP>::DT <= 2, "chunks of a row");
+    const unsigned t = (unsigned)(unsigned long long)(__attribute__((address_space(3))) const char*)tile + k0 * RB + (p & 1) * 8;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int d = 0; d < XaTile<DP>::DT; ++d) at[i][d] = t + 16 * ((d * 4 + rg * 2 + (p >> 1)) ^ xa_swz<RB>(k0 + 8 * i));
+  }
+};
+template <int DP, int ROW>
+__device__ __forceinline__ void xa_tr_frags(const XaTr<DP>& a, unsigned base, u32x4 (&f)[XaTile<DP>::DT]) {
+  constexpr int RB = XaTile<DP>::RB, DT = XaTile<DP>::DT, OFF = ROW * RB;
+  u32x2 lo[DT], hi[DT];
+  if constexpr (DT == 1) {
+    asm volatile("ds_read_b64_tr_b16 %0, %2 offset:%4\n\t"
+                 "ds_read_b64_tr_b16 %1, %3 offset:%5\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(lo[0]), "=&v"(hi[0])
+                 : "v"(a.at[0][0] + base), "v"(a.at[1][0] + base), "n"(OFF), "n"(OFF + 8 * RB) : "memory");
+  } else if constexpr (DT == 2) {
+    asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%8\n\t"
+                 "ds_read_b64_tr_b16 %1, %5 offset:%9\n\t"
+                 "ds_read_b64_tr_b16 %2, %6 offset:%8\n\t"
+                 "ds_read_b64_tr_b16 %3, %7 offset:%9\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1])
+                 : "v"(a.at[0][0] + base), "v"(a.at[1][0] + base),
+                   "v"(a.at[0][1] + base), "v"(a.at[1][1] + base), "n"(OFF), "n"(OFF + 8 * RB) : "memory");
+  } else if constexpr (DT == 3) {
+    asm volatile("ds_read_b64_tr_b16 %0, %6 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %1, %7 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %2, %8 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %5, %11 offset:%13\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2])
+                 : "v"(a.at[0][0] + base), "v"(a.at[1][0] + base),
+                   "v"(a.at[0][1] + base), "v"(a.at[1][1] + base),
+                   "v"(a.at[0][2] + base), "v"(a.at[1][2] + base), "n"(OFF), "n"(OFF + 8 * RB) : "memory");
+  } else {
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%16\n\t"
+                 "ds_read_b64_tr_b16 %1, %9 offset:%17\n\t"
+                 "ds_read_b64_tr_b16 %2, %10 offset:%16\n\t"
+                 "ds_read_b64_tr_b16 %3, %11 offset:%17\n\t"
+                 "ds_read_b64_tr_b16 %4, %12 offset:%16\n\t"
+                 "ds_read_b64_tr_b16 %5, %13 offset:%17\n\t"
+                 "ds_read_b64_tr_b16 %6, %14 offset:%16\n\t"
+                 "ds_read_b64_tr_b16 %7, %15 offset:%17\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
+                 : "v"(a.at[0][0] + base), "v"(a.at[1][0] + base),
+                   "v"(a.at[0][1] + base), "v"(a.at[1][1] + base),
+                   "v"(a.at[0][2] + base), "v"(a.at[1][2] + base),
+                   "v"(a.at[0][3] + base), "v"(a.at[1][3] + base), "n"(OFF), "n"(OFF + 8 * RB) : "memory");
+  }
+#pragma unroll
+  for (int d = 0; d < DT; ++d) f[d] = u32x4{lo[d][0], lo[d][1], hi[d][0], hi[d][1]};
 }
 
 // What every kernel of the family gets.  Strides in elements: batch, token, head.

@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaArgs A) {
   const char* vp = (const char*)((const T*)A.v + (long long)b * A.vs[0] + (long long)hk * A.vs[2]);
   const unsigned char* mp = A.mask ? A.mask + (long long)b * A.ms : nullptr;
   const int krow = (int)A.ks[1] * 2, vrow = (int)A.vs[1] * 2;    // bytes (host-checked: 64 rows stay below 2^31)
-  const int srow = wave * RPI + lane / NC, sc = (lane % NC) ^ xa_swz(srow);
+  const int srow = wave * RPI + lane / NC, sc = (lane % NC) ^ xa_swz<RB>(srow);
   const unsigned dead = sc * 8 >= A.D ? XA_OOB : 0u;
   const unsigned koff = (unsigned)(srow * krow + sc * 16) | dead, voff = (unsigned)(srow * vrow + sc * 16) | dead;
   auto issue = [&](int t, u64 w, int buf) {
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaArgs A) {
   f32x16 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = xa_zero();
-
+  const XaTr<DP> tr(smem + TILE, lane);
   u64 w = 0;
   int byte = 0, buf = 0;
   if (t0 < t1) {
@@ -76,14 +76,15 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaArgs A) {
       issue(t + 1, wn, buf ^ 1);
       byte = mask_byte(t + 2);
     }
-    if (w) {
+    {
       const char* kt = smem + buf * 2 * TILE;
-      const char* vt = kt + TILE;
       f32x16 s[2] = {xa_zero(), xa_zero()};
+      
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int u = 0; u < 2; ++u) s[u] = xa_mma<T>(xa_frag<DP>(kt, 32 * u, ks, lane), fq[ks], s[u]);
+      
       if (w != ~0ull) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -116,12 +117,17 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaArgs A) {
           s[u][r] = xa_exp2(__builtin_fmaf(s[u][r], c, -mc));
           sum += s[u][r];
         }
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb) {
+      
+      auto add = [&](auto kb_) {
+        constexpr int kb = decltype(kb_)::value;
+        u32x4 fv[DT];
+        xa_tr_frags<DP, kb * 16>(tr, buf * 2 * TILE, fv);
         const u32x4 p = xa_as_b<T>(s[kb >> 1], kb & 1);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(xa_tr_frag<DP>(vt, kb * 16, d, lane), p, acc[d]);
-      }
+        for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(fv[d], p, acc[d]);
+      };
+      add(XaInt<0>{}), add(XaInt<1>{}), add(XaInt<2>{}), add(XaInt<3>{});
+      
     }
     w = wn;
     buf ^= 1;
@@ -192,13 +198,14 @@ __global__ __launch_bounds__(256, 1) void xattn_token_kernel(XaArgs A) {
   const int krow = (int)A.ks[1] * 2, vrow = (int)A.vs[1] * 2;
   const int srow = lane / NC;
   char* const base = smem + wave * 4 * TILE;
+  const XaTr<DP> tr(base + TILE, lane);
   // (a wave's DMA instruction i fills rows i * RPI ..; with RPI = 4 the swizzle of odd i differs)
   auto issue = [&](int t, unsigned w, int buf) {
     const __amdgpu_buffer_rsrc_t rk = xa_rsrc(kp + (long long)t * 32 * krow), rv = xa_rsrc(vp + (long long)t * 32 * vrow);
     char* dst = base + buf * 2 * TILE;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int r = srow + i * RPI, sc = (lane % NC) ^ xa_swz(r);
+      const int r = srow + i * RPI, sc = (lane % NC) ^ xa_swz<RB>(r);
       const unsigned bad = ((w >> r) & 1) && sc * 8 < A.D ? 0u : XA_OOB;
       xa_dma16(rk, (unsigned)(srow * krow + sc * 16) | bad, i * RPI * krow, dst + i * RPI * RB);
       xa_dma16(rv, (unsigned)(srow * vrow + sc * 16) | bad, i * RPI * vrow, dst + TILE + i * RPI * RB);
@@ -226,7 +233,6 @@ __global__ __launch_bounds__(256, 1) void xattn_token_kernel(XaArgs A) {
     for (int t = t0; t < t1; t += 4) {
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
       const char* kt = base + buf * 2 * TILE;
-      const char* vt = kt + TILE;
       f32x16 s = xa_zero();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) s = xa_mma<T>(xa_frag<DP>(kt, 0, ks, lane), fq[ks], s);
@@ -255,12 +261,15 @@ __global__ __launch_bounds__(256, 1) void xattn_token_kernel(XaArgs A) {
         s[r] = xa_exp2(__builtin_fmaf(s[r], c, -mc));
         sum += s[r];
       }
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
+      auto add = [&](auto kb_) {
+        constexpr int kb = decltype(kb_)::value;
+        u32x4 fv[DT];
+        xa_tr_frags<DP, kb * 16>(tr, buf * 2 * TILE, fv);
         const u32x4 p = xa_as_b<T>(s, kb);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(xa_tr_frag<DP>(vt, kb * 16, d, lane), p, acc[d]);
-      }
+        for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(fv[d], p, acc[d]);
+      };
+      add(XaInt<0>{}), add(XaInt<1>{});
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // this stage has been read
       const unsigned w2 = word(t + 8, byte);
       byte = mask_byte(t + 12);

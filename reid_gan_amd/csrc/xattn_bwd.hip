@@ -83,7 +83,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
   const char* vp = (const char*)((const T*)A.v + (long long)b * A.vs[0] + (long long)hk * A.vs[2]);
   const unsigned char* mp = A.mask ? A.mask + (long long)b * A.ms : nullptr;
   const int krow = (int)A.ks[1] * 2, vrow = (int)A.vs[1] * 2;
-  const int srow = wave * RPI + lane / NC, sc = (lane % NC) ^ xa_swz(srow);
+  const int srow = wave * RPI + lane / NC, sc = (lane % NC) ^ xa_swz<RB>(srow);
   const unsigned dead = sc * 8 >= A.D ? XA_OOB : 0u;
   const unsigned koff = (unsigned)(srow * krow + sc * 16) | dead, voff = (unsigned)(srow * vrow + sc * 16) | dead;
   auto issue = [&](int t, u64 w, int buf) {
@@ -105,6 +105,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
   f32x16 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = xa_zero();
+  const XaTr<DP> tr(smem, lane);
   u64 w = 0;
   int byte = 0, buf = 0;
   if (t0 < t1) {
@@ -125,8 +126,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
     if (w) {
       const char* kt = smem + buf * 2 * TILE;
       const char* vt = kt + TILE;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      auto keys32 = [&](auto u_) {
+        constexpr int u = decltype(u_)::value;
         f32x16 s = xa_zero(), dp = xa_zero();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -151,13 +152,17 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] *= es;
         }
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        auto add = [&](auto kb_) {
+          constexpr int kb = decltype(kb_)::value;
+          u32x4 fk[DT];
+          xa_tr_frags<DP, u * 32 + kb * 16>(tr, buf * 2 * TILE, fk);
           const u32x4 f = xa_as_b<T>(s, kb);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(xa_tr_frag<DP>(kt, u * 32 + kb * 16, d, lane), f, acc[d]);
-        }
-      }
+          for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(fk[d], f, acc[d]);
+        };
+        add(XaInt<0>{}), add(XaInt<1>{});
+      };
+      keys32(XaInt<0>{}), keys32(XaInt<1>{});
     }
     w = wn;
     buf ^= 1;
@@ -224,7 +229,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xattn_dkv_kernel(XaArgs
   const __amdgpu_buffer_rsrc_t rq = xa_rsrc(qp), rg = xa_rsrc(gp);   // (host-checked: the heads of a group stay below 2^31 bytes)
   const __amdgpu_buffer_rsrc_t rl = xa_rsrc(A.lse2 + (long long)head * A.rows), rd = xa_rsrc(A.delta + (long long)head * A.rows);
   const int qrow = (int)A.qs[1] * 2, qhead = (int)A.qs[2] * 2, grow = (int)A.gs[1] * 2, ghead = (int)A.gs[2] * 2;
-  const int srow = wave * RPI + lane / NC, sc = (lane % NC) ^ xa_swz(srow);
+  const int srow = wave * RPI + lane / NC, sc = (lane % NC) ^ xa_swz<RB>(srow);
   const unsigned dead = sc * 8 >= A.D ? XA_OOB : 0u;
   const float inv_lq = 1.f / (float)A.Lq;
   auto issue = [&](int t, int buf) {
@@ -250,6 +255,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xattn_dkv_kernel(XaArgs
   f32x16 dv[DT], dk[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) dv[d] = dk[d] = xa_zero();
+  const XaTr<DP> tr(smem, lane);
   int buf = 0;
   if (t0 < t1) issue(t0, 0);
   for (int t = t0; t < t1; ++t) {
@@ -260,8 +266,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xattn_dkv_kernel(XaArgs
     const char* qt = smem + buf * STAGE;
     const char* gt = qt + TILE;
     const float* rowv = reinterpret_cast<const float*>(qt + 2 * TILE);
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    auto rows32 = [&](auto u_) {
+      constexpr int u = decltype(u_)::value;
       f32x16 s = xa_zero(), dp = xa_zero();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -286,16 +292,21 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xattn_dkv_kernel(XaArgs
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] *= es;
       }
+      auto add = [&](auto kb_) {
+        constexpr int kb = decltype(kb_)::value;
+        u32x4 fg[DT], fq[DT];
+        xa_tr_frags<DP, u * 32 + kb * 16>(tr, buf * STAGE + TILE, fg);
+        const u32x4 fp = xa_as_b<T>(s, kb);
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const u32x4 fp = xa_as_b<T>(s, kb), fs = xa_as_b<T>(dp, kb);
+        for (int d = 0; d < DT; ++d) dv[d] = xa_mma<T>(fg[d], fp, dv[d]);
+        xa_tr_frags<DP, u * 32 + kb * 16>(tr, buf * STAGE, fq);
+        const u32x4 fs = xa_as_b<T>(dp, kb);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          dv[d] = xa_mma<T>(xa_tr_frag<DP>(gt, u * 32 + kb * 16, d, lane), fp, dv[d]);
-          dk[d] = xa_mma<T>(xa_tr_frag<DP>(qt, u * 32 + kb * 16, d, lane), fs, dk[d]);
-        }
-      }
-    }
+        for (int d = 0; d < DT; ++d) dk[d] = xa_mma<T>(fq[d], fs, dk[d]);
+      };
+      add(XaInt<0>{}), add(XaInt<1>{});
+    };
+    rows32(XaInt<0>{}), rows32(XaInt<1>{});
     buf ^= 1;
   }
   if (key >= A.Lk) return;

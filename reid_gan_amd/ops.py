@@ -5,7 +5,6 @@ computation below is a hand-written HIP kernel in libried_gan.so.
 """
 from __future__ import annotations
 
-import contextlib
 import struct
 from dataclasses import dataclass
 from functools import lru_cache
@@ -16,7 +15,6 @@ import torch
 from ._lib import lib
 
 BF16 = torch.bfloat16
-_HERE = contextlib.nullcontext()
 
 
 def _stream() -> int:
@@ -744,33 +742,50 @@ def ssim_bwd(a, ref, gmap, scale, da, scale_dev=None, accumulate=False):
 TOKEN_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 _XATTN = struct.Struct("=12q24q8qd")           # ried_xattn_t
+_NO_STRIDES = (0,) * 12
 
 
-def on_device(t: torch.Tensor):
-    """Context in which `t`'s device is the current one."""
-    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+_raw_stream = torch._C._cuda_getCurrentRawStream      # the address alone, without the Stream object
 
 
-def layer_norm_fwd(x: torch.Tensor, w, b, y: torch.Tensor, mean, rstd, eps: float):
-    """y = (x - mean) * rstd * w + b over the rows of x [rows][C] (row strides x.stride(0), y.stride(0)); w, b may be
-    None; mean, rstd: fp32 [rows] or None."""
-    with on_device(x):
-        lib.ried_layer_norm_fwd(x.data_ptr(), x.stride(0), _p(w), _p(b), y.data_ptr(), y.stride(0), _p(mean), _p(rstd),
-                                x.shape[0], x.shape[1], eps, TOKEN_TYPES[x.dtype], 0 if w is None else TOKEN_TYPES[w.dtype],
-                                _stream())
+def _on_device(t: torch.Tensor, entry, *args):
+    """entry(*args, stream) with `t`'s device current, on that device's current stream."""
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        entry(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            entry(*args, _raw_stream(index))
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.shape[-1] if t.is_contiguous() else t.stride(0)
+
+
+def layer_norm_fwd(x: torch.Tensor, w, b, y: torch.Tensor, stats, eps: float):
+    """y = (x - mean) * rstd * w + b over the last axis; x and y: contiguous tensors of one shape, or [rows][C] with any row
+    strides; w, b may be None; stats: fp32 [2][rows] that receives mean and rstd, or None."""
+    C, wt = x.shape[-1], w if w is not None else b
+    rows = x.numel() // C
+    at = 0 if stats is None else stats.data_ptr()
+    _on_device(x, lib.ried_layer_norm_fwd, x.data_ptr(), _row_stride(x), _p(w), _p(b), y.data_ptr(), _row_stride(y), at or None,
+               at + 4 * rows if at else None, rows, C, eps, TOKEN_TYPES[x.dtype], 0 if wt is None else TOKEN_TYPES[wt.dtype])
 
 
 def layer_norm_bwd_scratch_floats(rows: int, C: int, dtype: torch.dtype) -> int:
     return lib.ried_layer_norm_bwd_scratch_floats(rows, C, TOKEN_TYPES[dtype])
 
 
-def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, w, mean, rstd, dx: torch.Tensor, dw, db, scratch):
-    """dx, and the parameter gradients dw = sum dy * xh, db = sum dy (None: not wanted) of layer_norm_fwd."""
+def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, w, stats: torch.Tensor, dx: torch.Tensor, dw, db, scratch):
+    """dx, and the parameter gradients dw = sum dy * xh, db = sum dy (None: not wanted) of layer_norm_fwd; scratch:
+    layer_norm_bwd_scratch_floats() floats where a parameter gradient is wanted."""
     wt = w if w is not None else dw if dw is not None else db
-    with on_device(x):
-        lib.ried_layer_norm_bwd(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), _p(w), mean.data_ptr(),
-                                rstd.data_ptr(), dx.data_ptr(), dx.stride(0), _p(dw), _p(db), _p(scratch), x.shape[0],
-                                x.shape[1], TOKEN_TYPES[x.dtype], 0 if wt is None else TOKEN_TYPES[wt.dtype], _stream())
+    C = x.shape[-1]
+    rows = x.numel() // C
+    at = stats.data_ptr()
+    _on_device(x, lib.ried_layer_norm_bwd, dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x), _p(w), at, at + 4 * rows,
+               dx.data_ptr(), _row_stride(dx), _p(dw), _p(db), _p(scratch), rows, C, TOKEN_TYPES[x.dtype],
+               0 if wt is None else TOKEN_TYPES[wt.dtype])
 
 
 def rotary(x: torch.Tensor, y: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sections, interleaved: bool,
@@ -779,24 +794,25 @@ def rotary(x: torch.Tensor, y: torch.Tensor, positions: torch.Tensor, freqs: tor
     B, L, H, D = x.shape
     s = tuple(sections) + (0,) * (4 - len(sections))
     xs, ys, ps = x.stride(), y.stride(), positions.stride()
-    with on_device(x):
-        lib.ried_rotary(x.data_ptr(), xs[0], xs[1], xs[2], y.data_ptr(), ys[0], ys[1], ys[2], positions.data_ptr(),
-                        POSITION_TYPES[positions.dtype], ps[0], ps[1], ps[2], freqs.data_ptr(), s[0], s[1], s[2], s[3],
-                        B, L, H, D, interleaved, inverse, TOKEN_TYPES[x.dtype], _stream())
+    _on_device(x, lib.ried_rotary, x.data_ptr(), xs[0], xs[1], xs[2], y.data_ptr(), ys[0], ys[1], ys[2],
+               positions.data_ptr(), POSITION_TYPES[positions.dtype], ps[0], ps[1], ps[2], freqs.data_ptr(), s[0], s[1], s[2],
+               s[3], B, L, H, D, interleaved, inverse, TOKEN_TYPES[x.dtype])
 
 
 def _xattn_desc(q, k, v, o, lse, lengths, key_mask, scratch, scale, dout=None, dq=None, dk=None, dv=None) -> bytes:
-    B, Lq, H, D = q.shape
-    zero = (0, 0, 0)
-    back = dout is not None
+    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), o.stride()
+    (B, Lq, H, D), (_, Lk, G, _) = q.shape, k.shape
+    if dout is None:
+        back, strides = (0, 0, 0, 0), _NO_STRIDES
+    else:
+        back = (dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+        strides = dout.stride()[:3] + dq.stride()[:3] + dk.stride()[:3] + dv.stride()[:3]
     return _XATTN.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(),
         0 if lengths is None else lengths.data_ptr(), 0 if key_mask is None else key_mask.data_ptr(),
-        0 if scratch is None else scratch.data_ptr(), *((t.data_ptr() for t in (dout, dq, dk, dv)) if back else (0, 0, 0, 0)),
-        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3],
-        *(dout.stride()[:3] if back else zero), *(dq.stride()[:3] if back else zero), *(dk.stride()[:3] if back else zero),
-        *(dv.stride()[:3] if back else zero), 0 if key_mask is None else key_mask.stride(0), B, Lq, k.shape[1], H, k.shape[2],
-        D, TOKEN_TYPES[q.dtype], scale)
+        0 if scratch is None else scratch.data_ptr(), *back, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+        os_[0], os_[1], os_[2], *strides, 0 if key_mask is None else key_mask.stride(0), B, Lq, Lk, H, G, D,
+        TOKEN_TYPES[q.dtype], scale)
 
 
 @lru_cache(maxsize=4096)
@@ -812,20 +828,17 @@ def xattn_bwd_scratch_floats(batch: int, queries: int, keys: int, heads: int, gr
 def xattn_fwd(q, k, v, out, lse, scale: float, lengths=None, key_mask=None, scratch=None):
     """out [B][queries][heads][D] = attention of q over k, v [B][keys][key heads][D]; lse fp32 [B][heads][queries] or
     None; lengths int32 [B], key_mask one byte per [B][keys]; scratch: xattn_fwd_scratch_floats() floats."""
-    with on_device(q):
-        lib.ried_xattn_fwd(_xattn_desc(q, k, v, out, lse, lengths, key_mask, scratch, scale), _stream())
+    _on_device(q, lib.ried_xattn_fwd, _xattn_desc(q, k, v, out, lse, lengths, key_mask, scratch, scale))
 
 
 def xattn_bwd(dout, q, k, v, out, lse, dq, dk, dv, scale: float, scratch, lengths=None, key_mask=None):
     """dq, dk, dv (all written) of xattn_fwd; scratch: xattn_bwd_scratch_floats() floats."""
-    with on_device(q):
-        lib.ried_xattn_bwd(_xattn_desc(q, k, v, out, lse, lengths, key_mask, scratch, scale, dout, dq, dk, dv), _stream())
+    _on_device(q, lib.ried_xattn_bwd, _xattn_desc(q, k, v, out, lse, lengths, key_mask, scratch, scale, dout, dq, dk, dv))
 
 
 def adamw_jobs(jobs, blockmap, grads, first, steps, coef, lr, b1, b2, eps, weight_decay, dtype: torch.dtype, state_bits: int):
     """One AdamW step over the tensors of a job table (reid_gan_amd.optim builds it).  grads, first: host arrays
     (array('q') of addresses, array('i'))."""
-    with on_device(jobs):
-        lib.ried_adamw_jobs(jobs.data_ptr(), blockmap.data_ptr(), grads.buffer_info()[0], first.buffer_info()[0], len(grads),
-                            steps.data_ptr(), coef.data_ptr(), lr, b1, b2, eps, weight_decay, TOKEN_TYPES[dtype], state_bits,
-                            _stream())
+    _on_device(jobs, lib.ried_adamw_jobs, jobs.data_ptr(), blockmap.data_ptr(), grads.buffer_info()[0],
+               first.buffer_info()[0], len(grads), steps.data_ptr(), coef.data_ptr(), lr, b1, b2, eps, weight_decay,
+               TOKEN_TYPES[dtype], state_bits)

@@ -132,7 +132,7 @@ def test_layer_norm_views_and_rows_it_must_not_touch():
     one = normal(g, 64, to=BF16)
     assert torch.equal(attention.layer_norm(one), attention.layer_norm(one[None])[0])
     out = torch.full((12, 80), 7.0, dtype=BF16, device=DEV)
-    ops.layer_norm_fwd(x[:, :64], None, None, out[2:11, 8:72], None, None, 1e-5)
+    ops.layer_norm_fwd(x[:, :64], None, None, out[2:11, 8:72], None, 1e-5)
     assert torch.equal(out[2:11, 8:72], attention.layer_norm(x[:, :64]))
     out[2:11, 8:72] = 7.0
     assert bool((out == 7.0).all())
@@ -501,19 +501,19 @@ def test_captured_forward_and_backward():
     pos = torch.randint(0, 500, (B, Lq, 3), generator=g, device=DEV)
     dout = normal(g, B, Lq, H, D, to=BF16)
     like = lambda t: torch.empty_like(t)
-    y, mean, rstd, q, out, dq, dk, dv, dy, dx = like(x), *torch.empty(2, B * Lq, device=DEV), like(dout), like(dout), like(dout), like(k), like(v), like(x), like(x)
+    y, stats, q, out, dq, dk, dv, dy, dx = like(x), torch.empty(2, B * Lq, device=DEV), like(dout), like(dout), like(dout), like(k), like(v), like(x), like(x)
     lse, dw, db = torch.empty(B, H, Lq, device=DEV), like(w), like(b)
     s1 = torch.empty(max(1, ops.xattn_fwd_scratch_floats(B, Lq, Lk, H, Hk, D)), device=DEV)
     s2 = torch.empty(ops.xattn_bwd_scratch_floats(B, Lq, Lk, H, Hk, D), device=DEV)
     s3 = torch.empty(ops.layer_norm_bwd_scratch_floats(B * Lq, C, BF16), device=DEV)
 
     def step():
-        ops.layer_norm_fwd(x, w, b, y, mean, rstd, 1e-5)
+        ops.layer_norm_fwd(x, w, b, y, stats, 1e-5)
         ops.rotary(y.view(B, Lq, H, D), q, pos, freqs, sections, False, False)
         ops.xattn_fwd(q, k, v, out, lse, 0.125, scratch=s1)
         ops.xattn_bwd(dout, q, k, v, out, lse, dq, dk, dv, 0.125, s2)
         ops.rotary(dq, dy.view(B, Lq, H, D), pos, freqs, sections, False, True)
-        ops.layer_norm_bwd(dy, x, w, mean, rstd, dx, dw, db, s3)
+        ops.layer_norm_bwd(dy, x, w, stats, dx, dw, db, s3)
     results = (out, dx, dw, db, dk, dv)
     step()
     torch.cuda.synchronize()

@@ -71,78 +71,104 @@ __device__ __forceinline__ unsigned to_codes(const float (&f)[4], float& scale) 
   return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], u, true);
 }
 
-template <typename T, bool SMALL>
-__global__ __launch_bounds__(256) void adamw_kernel(AdamwGrads G, const AdamwJob* __restrict__ jobs,
-                                                    const int* __restrict__ map, int first, const float* __restrict__ coef,
-                                                    AdamwConst K) {
+// FULL: all elements of the workgroup's chunk exist
+template <typename T, bool SMALL, bool FULL>
+__device__ __forceinline__ void adamw_body(const AdamwJob& J, const T* __restrict__ g, int chunk, float rate, float root,
+                                           const AdamwConst& K) {
 #pragma clang fp contract(off)
-  const int ti = map[2 * blockIdx.x], chunk = map[2 * blockIdx.x + 1];
-  const T* g = (const T*)G.g[ti - first];
-  if (g == nullptr) return;
-  const AdamwJob J = jobs[ti];
   T* p = (T*)J.p;
-  const float rate = coef[2 * ti], root = coef[2 * ti + 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long long e0 = (long long)chunk * ADAMW_CHUNK + wave * 1024;
-  float pv[4][4], gv[4][4];
+  TokVec<T, 4> pr[4], gr[4];
+  f32x4 mr[4], vr[4];
   unsigned mc[4], rc[4];
-  float ms[4], rs[4], mv[4][4], vv[4][4];
+  float ms[4], rs[4];
   int n[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const long long at = e0 + k * ADAMW_BLOCK + lane * 4, left = J.n - at;
+    const long long at = e0 + k * ADAMW_BLOCK + lane * 4, left = J.n - at, blk = (e0 >> 8) + k;
     n[k] = left > 4 ? 4 : (int)left;
-    tok_load_n<T, 4>(p + at, n[k], pv[k]);
-    tok_load_n<T, 4>(g + at, n[k], gv[k]);
-    if constexpr (SMALL) {
-      const long long blk = (e0 >> 8) + k;
-      const bool live = blk * ADAMW_BLOCK < J.n;               // (uniform; the code buffers hold whole blocks)
-      mc[k] = live ? *(const unsigned*)((const char*)J.m + at) : 0u;
-      rc[k] = live ? *(const unsigned*)((const char*)J.v + at) : 0u;
-      ms[k] = live ? ((const float*)J.ms)[blk] : 0.f;
-      rs[k] = live ? ((const float*)J.vs)[blk] : 0.f;
+    // (the moments' buffers hold whole blocks of 256: no bound inside a block that exists)
+    const bool live = FULL || blk * ADAMW_BLOCK < J.n;
+    if constexpr (FULL) {
+      pr[k] = tok_raw<T, 4>(p + at);
+      gr[k] = tok_raw<T, 4>(g + at);
     } else {
-      tok_load_n<float, 4>((const float*)J.m + at, n[k], mv[k]);
-      tok_load_n<float, 4>((const float*)J.v + at, n[k], vv[k]);
+      pr[k] = tok_raw_n<T, 4>(p + at, n[k]);
+      gr[k] = tok_raw_n<T, 4>(g + at, n[k]);
+    }
+    if constexpr (SMALL) {
+      mc[k] = rc[k] = 0u;
+      ms[k] = rs[k] = 0.f;
+      if (live) {
+        mc[k] = *(const unsigned*)((const char*)J.m + at);
+        rc[k] = *(const unsigned*)((const char*)J.v + at);
+        ms[k] = ((const float*)J.ms)[blk];
+        rs[k] = ((const float*)J.vs)[blk];
+      }
+    } else {
+      mr[k] = vr[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (live) {
+        mr[k] = *(const f32x4*)((const float*)J.m + at);
+        vr[k] = *(const f32x4*)((const float*)J.v + at);
+      }
     }
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const long long at = e0 + k * ADAMW_BLOCK + lane * 4, blk = (e0 >> 8) + k;
-    float m[4], r[4], o[4];
+    const bool live = FULL || blk * ADAMW_BLOCK < J.n;
+    float pv[4], gv[4], m[4], v[4], r[4], o[4];
+    tok_up(pr[k], pv);
+    tok_up(gr[k], gv);
     if constexpr (SMALL) {
       from_codes(mc[k], ms[k], m);
       from_codes(rc[k], rs[k], r);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) vv[k][i] = r[i] * r[i];
+      for (int i = 0; i < 4; ++i) v[i] = r[i] * r[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { m[i] = mr[k][i]; v[i] = vr[k][i]; }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      m[i] = (SMALL ? m[i] : mv[k][i]) * K.b1 + gv[k][i] * K.c1;
-      vv[k][i] = vv[k][i] * K.b2 + (gv[k][i] * gv[k][i]) * K.c2;
-      r[i] = sqrtf(vv[k][i]);
-      o[i] = pv[k][i] * K.keep - rate * (m[i] / (r[i] * root + K.eps));
-      if (i >= n[k]) m[i] = r[i] = 0.f;
+      m[i] = m[i] * K.b1 + gv[i] * K.c1;
+      v[i] = v[i] * K.b2 + (gv[i] * gv[i]) * K.c2;
+      r[i] = sqrtf(v[i]);
+      o[i] = pv[i] * K.keep - rate * (m[i] / (r[i] * root + K.eps));
+      if (!FULL && i >= n[k]) m[i] = v[i] = r[i] = 0.f;           // padding of the last block
     }
     if constexpr (SMALL) {
-      float s;
-      const unsigned cm = to_codes<false>(m, s);
-      const bool live = blk * ADAMW_BLOCK < J.n;
+      float sm, sr;
+      const unsigned cm = to_codes<false>(m, sm), cr = to_codes<true>(r, sr);
       if (live) {
         *(unsigned*)((char*)J.m + at) = cm;
-        if (lane == 0) ((float*)J.ms)[blk] = s;
-      }
-      const unsigned cr = to_codes<true>(r, s);
-      if (live) {
         *(unsigned*)((char*)J.v + at) = cr;
-        if (lane == 0) ((float*)J.vs)[blk] = s;
+        if (lane == 0) {
+          ((float*)J.ms)[blk] = sm;
+          ((float*)J.vs)[blk] = sr;
+        }
       }
-    } else {
-      tok_store_n<float, 4>((float*)J.m + at, n[k], m);
-      tok_store_n<float, 4>((float*)J.v + at, n[k], vv[k]);
+    } else if (live) {
+      *(f32x4*)((float*)J.m + at) = f32x4{m[0], m[1], m[2], m[3]};
+      *(f32x4*)((float*)J.v + at) = f32x4{v[0], v[1], v[2], v[3]};
     }
-    tok_store_n<T, 4>(p + at, n[k], o);
+    if constexpr (FULL) tok_store<T, 4>(p + at, o);
+    else tok_store_n<T, 4>(p + at, n[k], o);
   }
+}
+
+template <typename T, bool SMALL>
+__global__ __launch_bounds__(256) void adamw_kernel(AdamwGrads G, const AdamwJob* __restrict__ jobs,
+                                                    const int* __restrict__ map, int first, const float* __restrict__ coef,
+                                                    AdamwConst K) {
+  const int ti = map[2 * blockIdx.x], chunk = map[2 * blockIdx.x + 1];
+  const T* g = (const T*)G.g[ti - first];
+  if (g == nullptr) return;
+  const AdamwJob J = jobs[ti];
+  const float rate = coef[2 * ti], root = coef[2 * ti + 1];
+  if ((long long)(chunk + 1) * ADAMW_CHUNK <= J.n) adamw_body<T, SMALL, true>(J, g, chunk, rate, root, K);
+  else adamw_body<T, SMALL, false>(J, g, chunk, rate, root, K);
 }
 
 extern "C" int ried_adamw_jobs(const long long* jobs, const int* map, const long long* grads_host, const int* first_host,

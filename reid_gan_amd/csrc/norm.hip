@@ -37,10 +37,15 @@ __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void ln_fwd_kernel(
   const T* xr = x + row * ldx;
   float f[NV][V];
   float s = 0.f;
+  TokVec<T, V> raw[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = (j * GS + l) * V;
-    tok_load_n<T, V>(xr + c, C - c, f[j]);
+    raw[j] = tok_raw_n<T, V>(xr + c, C - c);
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    tok_up(raw[j], f[j]);
 #pragma unroll
     for (int i = 0; i < V; ++i) s += f[j][i];
   }
@@ -110,14 +115,17 @@ __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void ln_bwd_kernel(
     const T* gr = dy + row * lddy;
     const float mu = live ? mean[row] : 0.f, rs = live ? rstd[row] : 0.f;
     float xh[NV][V], g[NV][V], s1 = 0.f, s2 = 0.f;
+    TokVec<T, V> rx[NV], rg[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * GS + l) * V, n = live ? C - c : 0;
-      tok_load_n<T, V>(xr + c, n, xh[j]);
-      tok_load_n<T, V>(gr + c, n, g[j]);
+      rx[j] = tok_raw_n<T, V>(xr + c, n);
+      rg[j] = tok_raw_n<T, V>(gr + c, n);
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      tok_up(rx[j], xh[j]);
+      tok_up(rg[j], g[j]);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         xh[j][i] = (xh[j][i] - mu) * rs;                          // (past the end: dy is 0 there)

@@ -7,6 +7,7 @@
 
 #define ROT_MAX_PAIRS 256
 #define ROT_TABLE 2048       // (token, pair) entries per block: 16 KB of LDS
+#define ROT_UNROLL 4         // chunks of 16 + 16 bytes a thread has in flight
 
 struct RotArgs {
   const void* x;
@@ -14,70 +15,98 @@ struct RotArgs {
   const void* pos;
   const double* freqs;
   long long xb, xl, xh, yb, yl, yh, pb, pl, pa;
-  long long tokens;
-  int L, H, D, pairs, s1, s2, s3, tpb, chunks;
+  int L, H, D, pairs, s1, s2, s3, tpb, lblocks, chunks;
   int ptype;                 // 0 int32, 1 int64, 2 fp32
-  float sign;
+  float sign, inv_pairs, inv_per, inv_chunks;
 };
 
-template <typename T, bool INTER>
+// WHOLE: the pairs are whole chunks, no load or store needs a bound
+template <typename T, bool INTER, bool WHOLE>
 __global__ __launch_bounds__(256) void rotary_kernel(RotArgs A) {
-  constexpr int V = TokType<T>::V;
-  __shared__ float cs[ROT_TABLE], sn[ROT_TABLE];
-  const long long t0 = (long long)blockIdx.x * A.tpb;
-  const int nt = A.tokens - t0 < A.tpb ? (int)(A.tokens - t0) : A.tpb;
+  constexpr int V = TokType<T>::V;                               // pairs per chunk
+  __shared__ __align__(16) float cs[ROT_TABLE], sn[ROT_TABLE];   // rows of `pitch` entries: whole chunks, read 16 bytes at a time
+  const int b = blockIdx.x / A.lblocks, l0 = (blockIdx.x - b * A.lblocks) * A.tpb;
+  const int nt = A.L - l0 < A.tpb ? A.L - l0 : A.tpb, pitch = A.chunks * V;
   for (int i = threadIdx.x; i < nt * A.pairs; i += 256) {
-    const int t = i / A.pairs, j = i - t * A.pairs;
-    const long long tok = t0 + t, b = tok / A.L, l = tok - b * A.L;
-    const long long at = b * A.pb + l * A.pl + ((j >= A.s1) + (j >= A.s2) + (j >= A.s3)) * A.pa;
+    int j;
+    const int t = fast_div(i, A.pairs, A.inv_pairs, j);
+    const long long at = b * A.pb + (long long)(l0 + t) * A.pl + ((j >= A.s1) + (j >= A.s2) + (j >= A.s3)) * A.pa;
     const double p = A.ptype == 0 ? (double)((const int*)A.pos)[at]
                    : A.ptype == 1 ? (double)((const long long*)A.pos)[at] : (double)((const float*)A.pos)[at];
     double turns = p * (A.freqs[j] * 0.15915494309189533577);
     turns -= rint(turns);
     float s, c;
     sincospif((float)(2.0 * turns), &s, &c);
-    cs[i] = c;
-    sn[i] = s * A.sign;
+    cs[t * pitch + j] = c;
+    sn[t * pitch + j] = s * A.sign;
   }
   __syncthreads();
-  const int per = A.H * A.chunks;
-  for (int i = threadIdx.x; i < nt * per; i += 256) {
-    const int t = i / per, r = i - t * per, h = r / A.chunks, j = (r - h * A.chunks) * V;   // pairs j .. j + V - 1
-    const long long tok = t0 + t, b = tok / A.L, l = tok - b * A.L;
-    const T* xp = (const T*)A.x + b * A.xb + l * A.xl + h * A.xh;
-    T* yp = (T*)A.y + b * A.yb + l * A.yl + h * A.yh;
-    const int n = A.pairs - j;
-    const float* tc = cs + t * A.pairs + j;
-    const float* ts = sn + t * A.pairs + j;
-    float a[V], c[V], p[V], q[V];
-    if constexpr (INTER) {
-      tok_load_n<T, V>(xp + 2 * j, 2 * n, a);
-      tok_load_n<T, V>(xp + 2 * j + V, 2 * n - V, c);
+  const T* xb = (const T*)A.x + b * A.xb + l0 * A.xl;
+  T* yb = (T*)A.y + b * A.yb + l0 * A.yl;
+  const int per = A.H * A.chunks, all = nt * per;
+  // A thread's chunks: loaded together, then turned and stored (in place a chunk is read before it is written, and no
+  // other thread's)
+  for (int i0 = threadIdx.x; i0 < all; i0 += 256 * ROT_UNROLL) {
+    TokVec<T, V> a[ROT_UNROLL], c[ROT_UNROLL];
+    int n[ROT_UNROLL], tab[ROT_UNROLL];
+    T* yp[ROT_UNROLL];
 #pragma unroll
-      for (int k = 0; k < V / 2; ++k) {
-        if (k < n) {
-          p[2 * k] = a[2 * k] * tc[k] - a[2 * k + 1] * ts[k];
-          p[2 * k + 1] = a[2 * k + 1] * tc[k] + a[2 * k] * ts[k];
-        }
-        if (k + V / 2 < n) {
-          q[2 * k] = c[2 * k] * tc[k + V / 2] - c[2 * k + 1] * ts[k + V / 2];
-          q[2 * k + 1] = c[2 * k + 1] * tc[k + V / 2] + c[2 * k] * ts[k + V / 2];
-        }
+    for (int u = 0; u < ROT_UNROLL; ++u) {
+      const int i = i0 + u * 256 < all ? i0 + u * 256 : i0;
+      int r, j;
+      const int t = fast_div(i, per, A.inv_per, r), h = fast_div(r, A.chunks, A.inv_chunks, j);
+      j *= V;
+      n[u] = i0 + u * 256 < all ? (WHOLE ? V : A.pairs - j) : 0;
+      tab[u] = t * pitch + j;
+      const T* xp = xb + t * A.xl + h * A.xh;
+      yp[u] = yb + t * A.yl + h * A.yh;
+      if constexpr (INTER) {
+        xp += 2 * j;
+        yp[u] += 2 * j;
+        a[u] = WHOLE ? tok_raw<T, V>(xp) : tok_raw_n<T, V>(xp, 2 * n[u]);
+        c[u] = WHOLE ? tok_raw<T, V>(xp + V) : tok_raw_n<T, V>(xp + V, 2 * n[u] - V);
+      } else {
+        xp += j;
+        yp[u] += j;
+        a[u] = WHOLE ? tok_raw<T, V>(xp) : tok_raw_n<T, V>(xp, n[u]);
+        c[u] = WHOLE ? tok_raw<T, V>(xp + A.pairs) : tok_raw_n<T, V>(xp + A.pairs, n[u]);
       }
-      tok_store_n<T, V>(yp + 2 * j, 2 * n, p);
-      tok_store_n<T, V>(yp + 2 * j + V, 2 * n - V, q);
-    } else {
-      tok_load_n<T, V>(xp + j, n, a);
-      tok_load_n<T, V>(xp + A.pairs + j, n, c);
+    }
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        if (k < n) {
-          p[k] = a[k] * tc[k] - c[k] * ts[k];
-          q[k] = c[k] * tc[k] + a[k] * ts[k];
-        }
+    for (int u = 0; u < ROT_UNROLL; ++u) {
+      if (WHOLE && n[u] == 0) break;                             // (n is V, or 0 from here on)
+      float tc[V], ts[V], p[V], q[V], x0[V], x1[V];
+      tok_up(a[u], x0);
+      tok_up(c[u], x1);
+#pragma unroll
+      for (int k = 0; k < V; k += 4) {
+        const f32x4 c4 = *reinterpret_cast<const f32x4*>(cs + tab[u] + k), s4 = *reinterpret_cast<const f32x4*>(sn + tab[u] + k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { tc[k + e] = c4[e]; ts[k + e] = s4[e]; }
       }
-      tok_store_n<T, V>(yp + j, n, p);
-      tok_store_n<T, V>(yp + A.pairs + j, n, q);
+      if constexpr (INTER) {
+#pragma unroll
+        for (int k = 0; k < V / 2; ++k) {
+          p[2 * k] = x0[2 * k] * tc[k] - x0[2 * k + 1] * ts[k];
+          p[2 * k + 1] = x0[2 * k + 1] * tc[k] + x0[2 * k] * ts[k];
+          q[2 * k] = x1[2 * k] * tc[k + V / 2] - x1[2 * k + 1] * ts[k + V / 2];
+          q[2 * k + 1] = x1[2 * k + 1] * tc[k + V / 2] + x1[2 * k] * ts[k + V / 2];
+        }
+        if (WHOLE) tok_store<T, V>(yp[u], p);
+        else tok_store_n<T, V>(yp[u], 2 * n[u], p);
+        if (WHOLE) tok_store<T, V>(yp[u] + V, q);
+        else tok_store_n<T, V>(yp[u] + V, 2 * n[u] - V, q);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          p[k] = x0[k] * tc[k] - x1[k] * ts[k];
+          q[k] = x1[k] * tc[k] + x0[k] * ts[k];
+        }
+        if (WHOLE) tok_store<T, V>(yp[u], p);
+        else tok_store_n<T, V>(yp[u], n[u], p);
+        if (WHOLE) tok_store<T, V>(yp[u] + A.pairs, q);
+        else tok_store_n<T, V>(yp[u] + A.pairs, n[u], q);
+      }
     }
   }
   // channels behind the rotated ones pass through
@@ -85,8 +114,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotArgs A) {
   if (rest > 0 && A.x != (const void*)A.y) {
     for (int i = threadIdx.x; i < nt * A.H * rest; i += 256) {
       const int t = i / (A.H * rest), r = i - t * (A.H * rest), h = r / rest, d = 2 * A.pairs + r - h * rest;
-      const long long tok = t0 + t, b = tok / A.L, l = tok - b * A.L;
-      ((T*)A.y)[b * A.yb + l * A.yl + h * A.yh + d] = ((const T*)A.x)[b * A.xb + l * A.xl + h * A.xh + d];
+      yb[t * A.yl + h * A.yh + d] = xb[t * A.xl + h * A.xh + d];
     }
   }
 }
@@ -107,23 +135,29 @@ extern "C" int ried_rotary(const void* x, long long xb, long long xl, long long 
   RotArgs A;
   A.x = x; A.y = y; A.pos = pos; A.freqs = freqs;
   A.xb = xb; A.xl = xl; A.xh = xh; A.yb = yb; A.yl = yl; A.yh = yh; A.pb = pb; A.pl = pl; A.pa = pa;
-  A.tokens = (long long)B * L;
   A.L = L; A.H = H; A.D = D; A.pairs = pairs; A.ptype = pos_type;
   A.s1 = s0; A.s2 = s0 + s1; A.s3 = s0 + s1 + s2;
   A.sign = inverse ? -1.f : 1.f;
   const int V = type == RIED_T_F32 ? 4 : 8;
   A.chunks = ceil_div(pairs, V);
-  // a block takes about 1024 chunks (four per thread), as many tokens as the table holds, and leaves 512 blocks to the chip
+  RIED_CHECK_ARG((long long)H * D < (1ll << 20), "ried_rotary: %d heads of %d channels are too many", H, D);
+  // a block takes about 1024 chunks (one round of four per thread) of one batch entry, as many tokens as the table holds, and
+  // leaves 512 blocks to the chip
   long long tpb = ceil_div(1024, H * A.chunks);
-  if (tpb > ROT_TABLE / pairs) tpb = ROT_TABLE / pairs;
-  const long long most = (A.tokens + 511) / 512;
+  if (tpb > ROT_TABLE / (A.chunks * V)) tpb = ROT_TABLE / (A.chunks * V);
+  const long long most = ((long long)B * L + 511) / 512;
   if (tpb > most) tpb = most;
   A.tpb = (int)(tpb < 1 ? 1 : tpb);
-  const long long blocks = (A.tokens + A.tpb - 1) / A.tpb;
+  A.lblocks = ceil_div(L, A.tpb);
+  A.inv_pairs = 1.f / (float)pairs;
+  A.inv_per = 1.f / (float)(H * A.chunks);
+  A.inv_chunks = 1.f / (float)A.chunks;
+  const long long blocks = (long long)B * A.lblocks;
   RIED_CHECK_ARG(blocks <= 0x7fffffffll, "ried_rotary: too many tokens");
   TOK_DISPATCH(type, T, {
-    if (interleaved) hipLaunchKernelGGL((rotary_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, stream, A);
-    else hipLaunchKernelGGL((rotary_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, stream, A);
+#define ROT_LAUNCH(INTER, WHOLE) hipLaunchKernelGGL((rotary_kernel<T, INTER, WHOLE>), dim3((unsigned)blocks), dim3(256), 0, stream, A)
+    if (pairs % V == 0) { if (interleaved) ROT_LAUNCH(true, true); else ROT_LAUNCH(false, true); }
+    else { if (interleaved) ROT_LAUNCH(true, false); else ROT_LAUNCH(false, false); }
   });
   RIED_CHECK_LAUNCH("ried_rotary");
   return RIED_OK;

@@ -30,28 +30,35 @@ template <typename T, int N> struct TokVec {
   T e[N];
 } __attribute__((packed, aligned(sizeof(T))));
 
+// Loads come in two steps - the elements as they lie, and their values - so that a kernel can have all its loads in
+// flight before the first is used (a conversion inside the branch of a partial load would wait for it there).
 template <typename T, int N>
-__device__ __forceinline__ void tok_load(const T* p, float (&f)[N]) {
-  const TokVec<T, N> v = *reinterpret_cast<const TokVec<T, N>*>(p);
+__device__ __forceinline__ TokVec<T, N> tok_raw(const T* p) { return *reinterpret_cast<const TokVec<T, N>*>(p); }
+// the first n of N (n <= 0: none); what is not there reads as zero
+template <typename T, int N>
+__device__ __forceinline__ TokVec<T, N> tok_raw_n(const T* p, int n) {
+  TokVec<T, N> v;
+  if (n >= N) {
+    v = tok_raw<T, N>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v.e[i] = i < n ? p[i] : (T)0;
+  }
+  return v;
+}
+template <typename T, int N>
+__device__ __forceinline__ void tok_up(const TokVec<T, N>& v, float (&f)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) f[i] = TokType<T>::up(v.e[i]);
 }
+template <typename T, int N>
+__device__ __forceinline__ void tok_load_n(const T* p, int n, float (&f)[N]) { tok_up(tok_raw_n<T, N>(p, n), f); }
 template <typename T, int N>
 __device__ __forceinline__ void tok_store(T* p, const float (&f)[N]) {
   TokVec<T, N> v;
 #pragma unroll
   for (int i = 0; i < N; ++i) v.e[i] = TokType<T>::down(f[i]);
   *reinterpret_cast<TokVec<T, N>*>(p) = v;
-}
-// the first n of N (n <= 0: none); what is not there reads as zero
-template <typename T, int N>
-__device__ __forceinline__ void tok_load_n(const T* p, int n, float (&f)[N]) {
-  if (n >= N) {
-    tok_load<T, N>(p, f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = i < n ? TokType<T>::up(p[i]) : 0.f;
-  }
 }
 template <typename T, int N>
 __device__ __forceinline__ void tok_store_n(T* p, int n, const float (&f)[N]) {

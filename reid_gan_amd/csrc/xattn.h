@@ -97,7 +97,7 @@ __device__ __forceinline__ u32x4 xa_frag(const char* tile, int rowbase, int ks, 
 // order).  Written in assembly, its wait included: the compiler cannot tell the transposing read from the DMA stage that
 // is being filled and would wait for that first, which puts a memory round trip into every tile.
 template <int DP> struct XaTr {
-  unsigned at[2][XaTile<DP>::DT];                                 // this lane's LDS addresses in the first tile: rows k0, k0 + 8
+  unsigned at[2][XaTile<DP>::DT];                                 // this lane's LDS addresses in a tile: rows k0, k0 + 8
   __device__ __forceinline__ XaTr(const char* tile, int lane) {
     constexpr int RB = XaTile<DP>::RB;
     const int h = lane >> 5, rg = (lane >> 4) & 1, q = (lane >> 2) & 3, p = lane & 3, k0 = 4 * h + q;
@@ -108,17 +108,24 @@ template <int DP> struct XaTr {
 #pragma unroll
       for (int d = 0; d < XaTile<DP>::DT; ++d) at[i][d] = t + 16 * ((d * 4 + rg * 2 + (p >> 1)) ^ xa_swz<RB>(k0 + 8 * i));
   }
+  __device__ __forceinline__ void move(int bytes) {               // to another tile
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int d = 0; d < XaTile<DP>::DT; ++d) at[i][d] += bytes;
+  }
 };
-template <int DP, int ROW>
-__device__ __forceinline__ void xa_tr_frags(const XaTr<DP>& a, unsigned base, u32x4 (&f)[XaTile<DP>::DT]) {
-  constexpr int RB = XaTile<DP>::RB, DT = XaTile<DP>::DT, OFF = ROW * RB;
+template <int DP, int ROW, int MORE = 0>                           // MORE: bytes from the tile that `a` points at
+__device__ __forceinline__ void xa_tr_frags(const XaTr<DP>& a, u32x4 (&f)[XaTile<DP>::DT]) {
+  constexpr int RB = XaTile<DP>::RB, DT = XaTile<DP>::DT, OFF = ROW * RB + MORE;
+  static_assert(OFF + 8 * RB < 65536, "LDS instruction offset");
   u32x2 lo[DT], hi[DT];
   if constexpr (DT == 1) {
     asm volatile("ds_read_b64_tr_b16 %0, %2 offset:%4\n\t"
                  "ds_read_b64_tr_b16 %1, %3 offset:%5\n\t"
                  "s_waitcnt lgkmcnt(0)"
                  : "=&v"(lo[0]), "=&v"(hi[0])
-                 : "v"(a.at[0][0] + base), "v"(a.at[1][0] + base), "n"(OFF), "n"(OFF + 8 * RB) : "memory");
+                 : "v"(a.at[0][0]), "v"(a.at[1][0]), "n"(OFF), "n"(OFF + 8 * RB) : "memory");
   } else if constexpr (DT == 2) {
     asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%8\n\t"
                  "ds_read_b64_tr_b16 %1, %5 offset:%9\n\t"
@@ -126,8 +133,8 @@ __device__ __forceinline__ void xa_tr_frags(const XaTr<DP>& a, unsigned base, u3
                  "ds_read_b64_tr_b16 %3, %7 offset:%9\n\t"
                  "s_waitcnt lgkmcnt(0)"
                  : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1])
-                 : "v"(a.at[0][0] + base), "v"(a.at[1][0] + base),
-                   "v"(a.at[0][1] + base), "v"(a.at[1][1] + base), "n"(OFF), "n"(OFF + 8 * RB) : "memory");
+                 : "v"(a.at[0][0]), "v"(a.at[1][0]),
+                   "v"(a.at[0][1]), "v"(a.at[1][1]), "n"(OFF), "n"(OFF + 8 * RB) : "memory");
   } else if constexpr (DT == 3) {
     asm volatile("ds_read_b64_tr_b16 %0, %6 offset:%12\n\t"
                  "ds_read_b64_tr_b16 %1, %7 offset:%13\n\t"
@@ -137,9 +144,9 @@ __device__ __forceinline__ void xa_tr_frags(const XaTr<DP>& a, unsigned base, u3
                  "ds_read_b64_tr_b16 %5, %11 offset:%13\n\t"
                  "s_waitcnt lgkmcnt(0)"
                  : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2])
-                 : "v"(a.at[0][0] + base), "v"(a.at[1][0] + base),
-                   "v"(a.at[0][1] + base), "v"(a.at[1][1] + base),
-                   "v"(a.at[0][2] + base), "v"(a.at[1][2] + base), "n"(OFF), "n"(OFF + 8 * RB) : "memory");
+                 : "v"(a.at[0][0]), "v"(a.at[1][0]),
+                   "v"(a.at[0][1]), "v"(a.at[1][1]),
+                   "v"(a.at[0][2]), "v"(a.at[1][2]), "n"(OFF), "n"(OFF + 8 * RB) : "memory");
   } else {
     asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%16\n\t"
                  "ds_read_b64_tr_b16 %1, %9 offset:%17\n\t"
@@ -151,10 +158,10 @@ __device__ __forceinline__ void xa_tr_frags(const XaTr<DP>& a, unsigned base, u3
                  "ds_read_b64_tr_b16 %7, %15 offset:%17\n\t"
                  "s_waitcnt lgkmcnt(0)"
                  : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
-                 : "v"(a.at[0][0] + base), "v"(a.at[1][0] + base),
-                   "v"(a.at[0][1] + base), "v"(a.at[1][1] + base),
-                   "v"(a.at[0][2] + base), "v"(a.at[1][2] + base),
-                   "v"(a.at[0][3] + base), "v"(a.at[1][3] + base), "n"(OFF), "n"(OFF + 8 * RB) : "memory");
+                 : "v"(a.at[0][0]), "v"(a.at[1][0]),
+                   "v"(a.at[0][1]), "v"(a.at[1][1]),
+                   "v"(a.at[0][2]), "v"(a.at[1][2]),
+                   "v"(a.at[0][3]), "v"(a.at[1][3]), "n"(OFF), "n"(OFF + 8 * RB) : "memory");
   }
 #pragma unroll
   for (int d = 0; d < DT; ++d) f[d] = u32x4{lo[d][0], lo[d][1], hi[d][0], hi[d][1]};

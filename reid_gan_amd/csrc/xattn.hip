@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaArgs A) {
   f32x16 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = xa_zero();
-  const XaTr<DP> tr(smem + TILE, lane);
+  XaTr<DP> tr(smem + TILE, lane);
   u64 w = 0;
   int byte = 0, buf = 0;
   if (t0 < t1) {
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaArgs A) {
       auto add = [&](auto kb_) {
         constexpr int kb = decltype(kb_)::value;
         u32x4 fv[DT];
-        xa_tr_frags<DP, kb * 16>(tr, buf * 2 * TILE, fv);
+        xa_tr_frags<DP, kb * 16>(tr, fv);
         const u32x4 p = xa_as_b<T>(s[kb >> 1], kb & 1);
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(fv[d], p, acc[d]);
@@ -130,6 +130,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaArgs A) {
       
     }
     w = wn;
+    tr.move(buf ? -2 * TILE : 2 * TILE);
     buf ^= 1;
   }
   float lo, hi;
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(256, 1) void xattn_token_kernel(XaArgs A) {
   const int krow = (int)A.ks[1] * 2, vrow = (int)A.vs[1] * 2;
   const int srow = lane / NC;
   char* const base = smem + wave * 4 * TILE;
-  const XaTr<DP> tr(base + TILE, lane);
+  XaTr<DP> tr(base + TILE, lane);
   // (a wave's DMA instruction i fills rows i * RPI ..; with RPI = 4 the swizzle of odd i differs)
   auto issue = [&](int t, unsigned w, int buf) {
     const __amdgpu_buffer_rsrc_t rk = xa_rsrc(kp + (long long)t * 32 * krow), rv = xa_rsrc(vp + (long long)t * 32 * vrow);
@@ -264,7 +265,7 @@ __global__ __launch_bounds__(256, 1) void xattn_token_kernel(XaArgs A) {
       auto add = [&](auto kb_) {
         constexpr int kb = decltype(kb_)::value;
         u32x4 fv[DT];
-        xa_tr_frags<DP, kb * 16>(tr, buf * 2 * TILE, fv);
+        xa_tr_frags<DP, kb * 16>(tr, fv);
         const u32x4 p = xa_as_b<T>(s, kb);
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(fv[d], p, acc[d]);
@@ -276,6 +277,7 @@ __global__ __launch_bounds__(256, 1) void xattn_token_kernel(XaArgs A) {
       issue(t + 8 < t1 ? t + 8 : t0, w2, buf);
       w = w1;
       w1 = w2;
+      tr.move(buf ? -2 * TILE : 2 * TILE);
       buf ^= 1;
     }
   }
@@ -331,34 +333,56 @@ __global__ __launch_bounds__(256, 1) void xattn_token_kernel(XaArgs A) {
   }
 }
 
-// joins the shares of the keys: a thread per row and 8 channels
+// joins the shares of the keys: a wave per row.  The shares' weights are formed by one lane each (up to 64 shares); 16 lanes
+// by 8 channels take every fourth share each, so a row's loads are in flight together, and the four sums are added.
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs A) {
-  const int chunks = A.D >> 3;
-  const long long all = (long long)A.B * A.Hkv * A.rows, i = blockIdx.x * 256ll + threadIdx.x;
-  if (i >= all * chunks) return;
-  const long long flat = i / chunks;
-  const int d = (int)(i - flat * chunks) * 8;
-  float top = -INFINITY;
-  for (int s = 0; s < A.nsplit; ++s) {
-    const float l = A.part_lse[s * all + flat];
-    top = l > top || l != l ? l : top;
-  }
-  float o[8] = {}, tot = 0.f;
-  for (int s = 0; s < A.nsplit; ++s) {
-    const float l = A.part_lse[s * all + flat], f = l == -INFINITY ? 0.f : xa_exp2((l - top) * XA_LOG2E);
-    const float* p = A.part + (s * all + flat) * A.D + d;
-    tot += f;
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const long long all = (long long)A.B * A.Hkv * A.rows, flat = blockIdx.x * 4ll + (threadIdx.x >> 6);
+  if (flat >= all) return;
+  const float l = lane < A.nsplit ? A.part_lse[lane * all + flat] : -INFINITY;
+  float top = l;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) o[k] += f == 0.f ? 0.f : p[k] * f;
+  for (int o = 32; o > 0; o >>= 1) {
+    const float x = __shfl_xor(top, o, 64);
+    top = x > top || x != x ? x : top;                            // (NaN wins)
   }
+  const float w = l == -INFINITY ? 0.f : xa_exp2((l - top) * XA_LOG2E);
+  const float tot = wave_sum(w);
+  float o[8] = {};
+  const bool has = c * 8 < A.D;
+  for (int s0 = 0; s0 < A.nsplit; s0 += 16) {                     // (the same trips for every lane: the weights change lanes)
+    f32x4 x[4], y[4];
+    float f[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int s = s0 + 4 * u + q;
+      f[u] = __shfl(w, s & 63, 64);
+      x[u] = y[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (has && s < A.nsplit && f[u] != 0.f) {                   // (a share without keys wrote zeros)
+        const float* p = A.part + (s * all + flat) * A.D + c * 8;
+        x[u] = *reinterpret_cast<const f32x4*>(p);
+        y[u] = *reinterpret_cast<const f32x4*>(p + 4);
+      } else {
+        f[u] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { o[k] += x[u][k] * f[u]; o[4 + k] += y[u][k] * f[u]; }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) o[k] = rows_sum(o[k]);
   const float inv = tot == 0.f ? 0.f : 1.f / tot;
   const int head = (int)(flat / A.rows), row = (int)(flat - (long long)head * A.rows);
   const int b = head / A.Hkv, hk = head % A.Hkv, g = row / A.Lq, qi = row - g * A.Lq;
-  if (d == 0 && A.lse) A.lse[flat] = tot == 0.f ? -INFINITY : top + __logf(tot);
-  T* op = (T*)A.out + (long long)b * A.os[0] + (long long)qi * A.os[1] + (long long)(hk * A.G + g) * A.os[2] + d;
-  *reinterpret_cast<u32x4*>(op) = u32x4{xa_pack<T>(o[0] * inv, o[1] * inv), xa_pack<T>(o[2] * inv, o[3] * inv),
-                                        xa_pack<T>(o[4] * inv, o[5] * inv), xa_pack<T>(o[6] * inv, o[7] * inv)};
+  if (lane == 0 && A.lse) A.lse[flat] = tot == 0.f ? -INFINITY : top + __logf(tot);
+  if (q == 0 && has) {
+    T* op = (T*)A.out + (long long)b * A.os[0] + (long long)qi * A.os[1] + (long long)(hk * A.G + g) * A.os[2] + c * 8;
+    *reinterpret_cast<u32x4*>(op) = u32x4{xa_pack<T>(o[0] * inv, o[1] * inv), xa_pack<T>(o[2] * inv, o[3] * inv),
+                                          xa_pack<T>(o[4] * inv, o[5] * inv), xa_pack<T>(o[6] * inv, o[7] * inv)};
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -448,7 +472,7 @@ static int xa_fwd_launch(const XaArgs& A, hipStream_t stream) {
     hipLaunchKernelGGL((xattn_fwd_kernel<T, DP>), dim3(grid), dim3(256), lds, stream, A);
   }
   if (A.nsplit > 1)
-    hipLaunchKernelGGL((xattn_join_kernel<T>), dim3(ceil_div((long long)A.B * A.Hkv * A.rows * (A.D >> 3), 256)), dim3(256), 0, stream, A);
+    hipLaunchKernelGGL((xattn_join_kernel<T>), dim3(ceil_div((long long)A.B * A.Hkv * A.rows, 4)), dim3(256), 0, stream, A);
   return RIED_OK;
 }
 template <typename T>

@@ -5,6 +5,23 @@
 // added with atomics: the order of every sum is fixed.
 #include "xattn.h"
 
+// Few keys (this many tiles of 64) leave roundings nothing to average out in, so two of them are avoided there.  Dl =
+// sum_c dO o = sum_j P dP: the stored o is rounded and was formed from rounded weights, which with two keys is off by as
+// much as dP - Dl is large (and with one key dS = 0 is all there is); it is formed from the scores instead, in a first pass
+// over the keys.  And what rounding P and dS to the type leaves over enters the products as a second operand.
+#ifndef XA_WANT_K
+#define XA_WANT_K (d.dim <= 64 ? 1024 : 256)
+#endif
+#define XA_FEW 4
+template <typename T> __device__ __forceinline__ u32x4 xa_rest(const f32x16& s, int which, u32x4 rounded) {
+  float f[8];
+  xa_unpack<T>(rounded, f);
+  f32x16 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = s[8 * which + i] - f[i];
+  return xa_as_b<T>(r, 0);
+}
+
 // fp16 products hold dS only between 2^-24 and 2^16 while P alone spans more: dS travels times a power of two, lowered
 // (and the sums with it) when a value would pass 2^15.  bf16 has fp32's range and needs none.
 template <typename T> struct XaRange {
@@ -29,7 +46,8 @@ __device__ __forceinline__ void xa_fit(float mx, float& es, f32x16 (&acc)[DT]) {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // dq: the forward kernel's tiling.  S^T = K Q^T and dP^T = V dO^T per 32 keys, dS^T is the B operand of dq^T += K^T dS^T.
-// Also leaves the rows' exponent base (lse in powers of two, +infinity for a row without keys) and Dl for the other kernel.
+// Also leaves for the other kernel what its exponents add (p_up - lse, in powers of two; -infinity for a row without keys)
+// and Dl.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
@@ -47,6 +65,9 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
   const T* qp = (const T*)A.q + (long long)b * A.qs[0] + (long long)qi * A.qs[1] + (long long)hq * A.qs[2];
   const T* gp = (const T*)A.dout + (long long)b * A.gs[0] + (long long)qi * A.gs[1] + (long long)hq * A.gs[2];
   const T* op = (const T*)A.o + (long long)b * A.os[0] + (long long)qi * A.os[1] + (long long)hq * A.os[2];
+  const int nk = xa_keys(A, b), ntile = (nk + 63) >> 6, per = (ntile + A.nsplit - 1) / A.nsplit;
+  const int t0 = split * per, t1 = t0 + per < ntile ? t0 + per : ntile;
+  const bool few = A.nsplit == 1 && ntile <= XA_FEW;
   u32x4 fq[KS], fg[KS];
   float delta = 0.f;
 #pragma unroll
@@ -56,14 +77,18 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
     const u32x4 none = {0, 0, 0, 0};
     fq[s] = ok ? *reinterpret_cast<const u32x4*>(qp + d) : none;
     fg[s] = ok ? *reinterpret_cast<const u32x4*>(gp + d) : none;
-    const u32x4 fo = ok ? *reinterpret_cast<const u32x4*>(op + d) : none;
-    float x[8], y[8];
-    xa_unpack<T>(fg[s], x);
-    xa_unpack<T>(fo, y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) delta += x[i] * y[i];
   }
-  {
+  if (!few) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = s * 16 + h * 8;
+      const u32x4 fo = live && d < A.D ? *reinterpret_cast<const u32x4*>(op + d) : u32x4{0, 0, 0, 0};
+      float x[8], y[8];
+      xa_unpack<T>(fg[s], x);
+      xa_unpack<T>(fo, y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta += x[i] * y[i];
+    }
     float lo, hi;
     xa_halves(delta, lo, hi);
     delta = lo + hi;
@@ -72,13 +97,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
   if (live) {
     const float l = A.lse[flat];
     lse2 = l == -INFINITY ? INFINITY : l * XA_LOG2E;
-    if (split == 0 && h == 0) {
-      A.lse2[flat] = lse2;
-      A.delta[flat] = delta;
-    }
   }
-  const int nk = xa_keys(A, b), ntile = (nk + 63) >> 6, per = (ntile + A.nsplit - 1) / A.nsplit;
-  const int t0 = split * per, t1 = t0 + per < ntile ? t0 + per : ntile;
   const char* kp = (const char*)((const T*)A.k + (long long)b * A.ks[0] + (long long)hk * A.ks[2]);
   const char* vp = (const char*)((const T*)A.v + (long long)b * A.vs[0] + (long long)hk * A.vs[2]);
   const unsigned char* mp = A.mask ? A.mask + (long long)b * A.ms : nullptr;
@@ -101,72 +120,105 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
     return mp && key < nk ? mp[key] : 0;
   };
   const float c = A.scale * XA_LOG2E;
+  XaTr<DP> tr(smem, lane);
+  // tiles f .. e - 1 through the two stages, `use` on each 32 keys of a tile
+  auto sweep = [&](int f, int e, auto use) {
+    u64 w = 0;
+    int byte = 0, buf = 0;
+    if (f < e) {
+      w = xa_word(nk - f * 64, mp != nullptr, mask_byte(f));
+      issue(f, w, 0);
+      byte = mask_byte(f + 1);
+    }
+    for (int t = f; t < e; ++t) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      u64 wn = 0;
+      if (t + 1 < e) {
+        wn = xa_word(nk - (t + 1) * 64, mp != nullptr, byte);
+        issue(t + 1, wn, buf ^ 1);
+        byte = mask_byte(t + 2);
+      }
+      if (w) {
+        const char* kt = smem + buf * 2 * TILE;
+        const char* vt = kt + TILE;
+        auto keys32 = [&](auto u_) {
+          constexpr int u = decltype(u_)::value;
+          f32x16 s = xa_zero(), dp = xa_zero();
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            s = xa_mma<T>(xa_frag<DP>(kt, 32 * u, ks, lane), fq[ks], s);
+            dp = xa_mma<T>(xa_frag<DP>(vt, 32 * u, ks, lane), fg[ks], dp);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = xa_exp2(__builtin_fmaf(s[r], c, -lse2));
+          if (w != ~0ull) {                                       // (a hidden key's score reads as 0, not as nothing)
+            const unsigned bits = (unsigned)(w >> (32 * u)) >> (4 * h);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = (bits >> (8 * (r >> 2) + (r & 3))) & 1 ? s[r] : 0.f;
+          }
+          use(u_, s, dp);
+        };
+        keys32(XaInt<0>{}), keys32(XaInt<1>{});
+      }
+      w = wn;
+      tr.move(buf ? -2 * TILE : 2 * TILE);
+      buf ^= 1;
+    }
+    tr.move(buf ? -2 * TILE : 0);
+  };
+  if (few) {
+    sweep(0, ntile, [&](auto, f32x16& p, f32x16& dp) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) delta += p[r] * dp[r];
+    });
+    float lo, hi;
+    xa_halves(delta, lo, hi);
+    delta = lo + hi;
+    __builtin_amdgcn_s_barrier();                                 // (the stages are free again)
+    asm volatile("" ::: "memory");
+  }
+  if (live && split == 0 && h == 0) {
+    A.lse2[flat] = XaRange<T>::p_up - lse2;
+    A.delta[flat] = delta;
+  }
   float es = XaRange<T>::on ? 0x1p24f : 1.f;
   f32x16 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = xa_zero();
-  const XaTr<DP> tr(smem, lane);
-  u64 w = 0;
-  int byte = 0, buf = 0;
-  if (t0 < t1) {
-    w = xa_word(nk - t0 * 64, mp != nullptr, mask_byte(t0));
-    issue(t0, w, 0);
-    byte = mask_byte(t0 + 1);
-  }
-  for (int t = t0; t < t1; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    u64 wn = 0;
-    if (t + 1 < t1) {
-      wn = xa_word(nk - (t + 1) * 64, mp != nullptr, byte);
-      issue(t + 1, wn, buf ^ 1);
-      byte = mask_byte(t + 2);
-    }
-    if (w) {
-      const char* kt = smem + buf * 2 * TILE;
-      const char* vt = kt + TILE;
-      auto keys32 = [&](auto u_) {
-        constexpr int u = decltype(u_)::value;
-        f32x16 s = xa_zero(), dp = xa_zero();
+  auto rows = [&](auto few_) {
+    sweep(t0, t1, [&](auto u_, f32x16& s, f32x16& dp) {
+      constexpr int u = decltype(u_)::value;
+      float mx = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          s = xa_mma<T>(xa_frag<DP>(kt, 32 * u, ks, lane), fq[ks], s);
-          dp = xa_mma<T>(xa_frag<DP>(vt, 32 * u, ks, lane), fg[ks], dp);
+      for (int r = 0; r < 16; ++r) {
+        s[r] *= dp[r] - delta;
+        if constexpr (XaRange<T>::on) mx = fmaxf(mx, fabsf(s[r]));
+      }
+      if constexpr (XaRange<T>::on) {
+        xa_fit<DT>(mx, es, acc);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= es;
+      }
+      auto add = [&](auto kb_) {
+        constexpr int kb = decltype(kb_)::value;
+        u32x4 fk[DT];
+        xa_tr_frags<DP, u * 32 + kb * 16>(tr, fk);
+        const u32x4 f = xa_as_b<T>(s, kb);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(fk[d], f, acc[d]);
+        if constexpr (decltype(few_)::value) {
+          const u32x4 rest = xa_rest<T>(s, kb, f);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(fk[d], rest, acc[d]);
         }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = xa_exp2(__builtin_fmaf(s[r], c, -lse2));
-        if (w != ~0ull) {                                         // (a hidden key's score reads as 0, not as nothing)
-          const unsigned bits = (unsigned)(w >> (32 * u)) >> (4 * h);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = (bits >> (8 * (r >> 2) + (r & 3))) & 1 ? s[r] : 0.f;
-        }
-        float mx = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[r] *= dp[r] - delta;
-          if constexpr (XaRange<T>::on) mx = fmaxf(mx, fabsf(s[r]));
-        }
-        if constexpr (XaRange<T>::on) {
-          xa_fit<DT>(mx, es, acc);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] *= es;
-        }
-        auto add = [&](auto kb_) {
-          constexpr int kb = decltype(kb_)::value;
-          u32x4 fk[DT];
-          xa_tr_frags<DP, u * 32 + kb * 16>(tr, buf * 2 * TILE, fk);
-          const u32x4 f = xa_as_b<T>(s, kb);
-#pragma unroll
-          for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(fk[d], f, acc[d]);
-        };
-        add(XaInt<0>{}), add(XaInt<1>{});
       };
-      keys32(XaInt<0>{}), keys32(XaInt<1>{});
-    }
-    w = wn;
-    buf ^= 1;
-  }
+      add(XaInt<0>{}), add(XaInt<1>{});
+    });
+  };
+  if (few) rows(XaInt<1>{});
+  else rows(XaInt<0>{});
   if (!live) return;
   const float f = A.scale / es;
   if (A.nsplit == 1) {
@@ -194,20 +246,26 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// dk, dv: a block owns 128 keys, a wave 32 of them (K and V fragments in registers), and walks tiles of 64 rows (Q, dO and
-// the rows' two numbers through LDS DMA, two stages).  S = Q K^T and dP = dO V^T have the row along the registers, so P
+// dk, dv: a block owns 64 keys and walks tiles of rows (Q, dO and the rows' two numbers through LDS DMA, two stages); a
+// wave takes 32 of the keys (K and V fragments in registers) and 64 rows of every tile, and the row groups are added
+// through LDS at the end.  Up to 64 channels a block has eight waves (four row groups, two waves per SIMD where the keys
+// give only one block per CU), above that the registers allow four.  S = Q K^T and dP = dO V^T have the row along the registers, so P
 // and dS are the B operands of dv^T += dO^T P and dk^T += Q^T dS as they stand.
 // ---------------------------------------------------------------------------------------------------------------------
+template <int DP>
+struct XaKv { static constexpr int NW = DP <= 64 ? 8 : 4, RG = NW / 2, ROWS = 64 * RG, STAGE = 2 * ROWS * XaTile<DP>::RB + 8 * ROWS; };
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xattn_dkv_kernel(XaArgs A) {
+__global__ __launch_bounds__(64 * XaKv<DP>::NW, XaKv<DP>::NW / 4) void xattn_dkv_kernel(XaArgs A) {
   constexpr int KS = XaTile<DP>::KS, DT = XaTile<DP>::DT, RB = XaTile<DP>::RB, NC = XaTile<DP>::NC, RPI = XaTile<DP>::RPI;
-  constexpr int TILE = 64 * RB, NI = 16 / RPI, STAGE = 2 * TILE + 512;
-  extern __shared__ __align__(16) char smem[];                    // [2][Q tile, dO tile, 64 lse2, 64 Dl]
+  constexpr int NW = XaKv<DP>::NW, RG = XaKv<DP>::RG, ROWS = XaKv<DP>::ROWS, TILE = ROWS * RB, NI = ROWS / NW / RPI, STAGE = XaKv<DP>::STAGE;
+  constexpr int EX = 2 * DT * 4 * 64;                             // vectors of four a wave hands over
+  static_assert((RG - 1) * 2 * EX * 16 <= 2 * STAGE, "the exchange reuses the stages");
+  extern __shared__ __align__(16) char smem[];                    // [2][Q tile, dO tile, ROWS lse2, ROWS Dl]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   int inner, head;
   xa_block(A.tiles * A.nsplit, A.B * A.Hkv, inner, head);
   const int b = head / A.Hkv, hk = head % A.Hkv, tile = inner % A.tiles, split = inner / A.tiles;
-  const int key = tile * 128 + wave * 32 + (lane & 31);
+  const int grp = wave >> 1, key = tile * 64 + (wave & 1) * 32 + (lane & 31);
   const int nk = xa_keys(A, b);
   const bool counts = key < nk && (!A.mask || A.mask[(long long)b * A.ms + key]);
   const T* kp = (const T*)A.k + (long long)b * A.ks[0] + (long long)key * A.ks[1] + (long long)hk * A.ks[2];
@@ -220,10 +278,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xattn_dkv_kernel(XaArgs
     fk[s] = ok ? *reinterpret_cast<const u32x4*>(kp + d) : u32x4{0, 0, 0, 0};
     fv[s] = ok ? *reinterpret_cast<const u32x4*>(vp + d) : u32x4{0, 0, 0, 0};
   }
-  const int ntile = (A.rows + 63) >> 6, per = (ntile + A.nsplit - 1) / A.nsplit;
+  const int ntile = (A.rows + ROWS - 1) / ROWS, per = (ntile + A.nsplit - 1) / A.nsplit;
   const int t0 = split * per;
   int t1 = t0 + per < ntile ? t0 + per : ntile;
-  if (tile * 128 >= nk) t1 = t0;                                  // no key here counts: zeros
+  if (tile * 64 >= nk) t1 = t0;                                   // no key here counts: zeros
   const char* qp = (const char*)((const T*)A.q + (long long)b * A.qs[0] + (long long)hk * A.G * A.qs[2]);
   const char* gp = (const char*)((const T*)A.dout + (long long)b * A.gs[0] + (long long)hk * A.G * A.gs[2]);
   const __amdgpu_buffer_rsrc_t rq = xa_rsrc(qp), rg = xa_rsrc(gp);   // (host-checked: the heads of a group stay below 2^31 bytes)
@@ -237,88 +295,129 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xattn_dkv_kernel(XaArgs
     char* dst = st + wave * RPI * RB;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int r = t * 64 + srow + i * 4 * RPI;
+      const int r = t * ROWS + srow + i * NW * RPI;
       int qi;
       const int g = fast_div(r, A.Lq, inv_lq, qi);
       const unsigned bad = (r < A.rows ? 0u : XA_OOB) | dead;
-      xa_dma16(rq, (unsigned)(qi * qrow + g * qhead + sc * 16) | bad, 0, dst + i * 4 * RPI * RB);
-      xa_dma16(rg, (unsigned)(qi * grow + g * ghead + sc * 16) | bad, 0, dst + TILE + i * 4 * RPI * RB);
+      xa_dma16(rq, (unsigned)(qi * qrow + g * qhead + sc * 16) | bad, 0, dst + i * NW * RPI * RB);
+      xa_dma16(rg, (unsigned)(qi * grow + g * ghead + sc * 16) | bad, 0, dst + TILE + i * NW * RPI * RB);
     }
-    const int r = t * 64 + lane;
+    const int part = wave % RG, r = t * ROWS + part * 64 + lane;
     const unsigned off = r < A.rows ? (unsigned)r * 4u : XA_OOB;
-    if (wave == 0) xa_dma4(rl, off, st + 2 * TILE);
-    if (wave == 1) xa_dma4(rd, off, st + 2 * TILE + 256);
+    if (wave < RG) xa_dma4(rl, off, st + 2 * TILE + part * 256);
+    else xa_dma4(rd, off, st + 2 * TILE + 4 * ROWS + part * 256);
   };
   const float c = A.scale * XA_LOG2E;
-  const float up = counts ? XaRange<T>::p_up : -INFINITY;         // (a hidden key's column stays out of the range below)
+  const bool few = nk <= 64 * XA_FEW;
   float es = XaRange<T>::on ? 0x1p9f : 1.f;                       // (times the 2^15 of P)
   f32x16 dv[DT], dk[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) dv[d] = dk[d] = xa_zero();
-  const XaTr<DP> tr(smem, lane);
-  int buf = 0;
-  if (t0 < t1) issue(t0, 0);
-  for (int t = t0; t < t1; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (t + 1 < t1) issue(t + 1, buf ^ 1);
-    const char* qt = smem + buf * STAGE;
-    const char* gt = qt + TILE;
-    const float* rowv = reinterpret_cast<const float*>(qt + 2 * TILE);
-    auto rows32 = [&](auto u_) {
-      constexpr int u = decltype(u_)::value;
-      f32x16 s = xa_zero(), dp = xa_zero();
+  XaTr<DP> tr(smem + grp * 64 * RB, lane);
+  auto rows = [&](auto few_) {
+    int buf = 0;
+    if (t0 < t1) issue(t0, 0);
+    for (int t = t0; t < t1; ++t) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (t + 1 < t1) issue(t + 1, buf ^ 1);
+      const char* qt = smem + buf * STAGE + grp * 64 * RB;
+      const char* gt = qt + TILE;
+      const float* rowv = reinterpret_cast<const float*>(smem + buf * STAGE + 2 * TILE) + grp * 64;
+      auto rows32 = [&](auto u_) {
+        constexpr int u = decltype(u_)::value;
+        f32x16 s = xa_zero(), dp = xa_zero();
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        s = xa_mma<T>(xa_frag<DP>(qt, 32 * u, ks, lane), fk[ks], s);
-        dp = xa_mma<T>(xa_frag<DP>(gt, 32 * u, ks, lane), fv[ks], dp);
-      }
-      float mx = 0.f;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4 l4 = *reinterpret_cast<const f32x4*>(rowv + 32 * u + 8 * q + 4 * h);
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(rowv + 64 + 32 * u + 8 * q + 4 * h);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 4 * q + i;
-          s[r] = xa_exp2(__builtin_fmaf(s[r], c, up - l4[i]));
-          dp[r] = s[r] * (dp[r] - d4[i]);
-          if constexpr (XaRange<T>::on) mx = fmaxf(mx, fabsf(dp[r]));
+        for (int ks = 0; ks < KS; ++ks) {
+          s = xa_mma<T>(xa_frag<DP>(qt, 32 * u, ks, lane), fk[ks], s);
+          dp = xa_mma<T>(xa_frag<DP>(gt, 32 * u, ks, lane), fv[ks], dp);
         }
-      }
-      if constexpr (XaRange<T>::on) {
-        xa_fit<DT>(mx, es, dk);
+        float mx = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] *= es;
-      }
-      auto add = [&](auto kb_) {
-        constexpr int kb = decltype(kb_)::value;
-        u32x4 fg[DT], fq[DT];
-        xa_tr_frags<DP, u * 32 + kb * 16>(tr, buf * STAGE + TILE, fg);
-        const u32x4 fp = xa_as_b<T>(s, kb);
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 l4 = *reinterpret_cast<const f32x4*>(rowv + 32 * u + 8 * q + 4 * h);
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(rowv + ROWS + 32 * u + 8 * q + 4 * h);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) dv[d] = xa_mma<T>(fg[d], fp, dv[d]);
-        xa_tr_frags<DP, u * 32 + kb * 16>(tr, buf * STAGE, fq);
-        const u32x4 fs = xa_as_b<T>(dp, kb);
+          for (int i = 0; i < 4; ++i) {
+            const int r = 4 * q + i;
+            s[r] = xa_exp2(__builtin_fmaf(s[r], c, l4[i]));
+            dp[r] = s[r] * (dp[r] - d4[i]);
+            if constexpr (XaRange<T>::on) mx = fmaxf(mx, fabsf(dp[r]));
+          }
+        }
+        if constexpr (XaRange<T>::on) {
+          xa_fit<DT>(counts ? mx : 0.f, es, dk);                    // (a hidden key's column is dropped: any size)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) dk[d] = xa_mma<T>(fq[d], fs, dk[d]);
+          for (int r = 0; r < 16; ++r) dp[r] *= es;
+        }
+        auto add = [&](auto kb_) {
+          constexpr int kb = decltype(kb_)::value;
+          u32x4 fg[DT], fq[DT];
+          xa_tr_frags<DP, u * 32 + kb * 16, TILE>(tr, fg);
+          const u32x4 fp = xa_as_b<T>(s, kb);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) dv[d] = xa_mma<T>(fg[d], fp, dv[d]);
+          if constexpr (decltype(few_)::value) {
+            const u32x4 rest = xa_rest<T>(s, kb, fp);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dv[d] = xa_mma<T>(fg[d], rest, dv[d]);
+          }
+          xa_tr_frags<DP, u * 32 + kb * 16>(tr, fq);
+          const u32x4 fs = xa_as_b<T>(dp, kb);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) dk[d] = xa_mma<T>(fq[d], fs, dk[d]);
+          if constexpr (decltype(few_)::value) {
+            const u32x4 rest = xa_rest<T>(dp, kb, fs);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dk[d] = xa_mma<T>(fq[d], rest, dk[d]);
+          }
+        };
+        add(XaInt<0>{}), add(XaInt<1>{});
       };
-      add(XaInt<0>{}), add(XaInt<1>{});
-    };
-    rows32(XaInt<0>{}), rows32(XaInt<1>{});
-    buf ^= 1;
-  }
-  if (key >= A.Lk) return;
-  // (a hidden key's column was computed from zeros and is dropped, whatever it holds)
-  const float fk_ = A.scale * XaRange<T>::p_down / es, fv_ = XaRange<T>::p_down;
-#pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      dk[d][r] = counts ? dk[d][r] * fk_ : 0.f;
-      dv[d][r] = counts ? dv[d][r] * fv_ : 0.f;
+      rows32(XaInt<0>{}), rows32(XaInt<1>{});
+      tr.move(buf ? -STAGE : STAGE);
+      buf ^= 1;
     }
+  };
+  if (few) rows(XaInt<1>{});
+  else rows(XaInt<0>{});
+  // the other row groups' sums go to the first group's waves, added in order
+  const float fk_ = A.scale * XaRange<T>::p_down / es, fv_ = XaRange<T>::p_down;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  f32x4* ex = reinterpret_cast<f32x4*>(smem) + (wave & 1) * EX + lane;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) {
+    dk[d] *= fk_;
+    dv[d] *= fv_;
+    if (grp) {
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        f32x4* to = ex + (grp - 1) * 2 * EX + (d * 4 + (r >> 2)) * 64;
+        to[0] = f32x4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
+        to[DT * 4 * 64] = f32x4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+      }
+    }
+  }
+  __syncthreads();
+  if (grp || key >= A.Lk) return;
+#pragma unroll
+  for (int o = 0; o < RG - 1; ++o)
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const f32x4* from = ex + o * 2 * EX + (d * 4 + (r >> 2)) * 64;
+        const f32x4 a = from[0], b = from[DT * 4 * 64];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { dk[d][r + i] += a[i]; dv[d][r + i] += b[i]; }
+      }
+  // (a hidden key's column was computed from zeros and is dropped, whatever it holds)
+  if (!counts) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d) dk[d] = dv[d] = xa_zero();
+  }
   if (A.nsplit == 1) {
     T* pk = (T*)A.dk + (long long)b * A.dks[0] + (long long)key * A.dks[1] + (long long)hk * A.dks[2];
     T* pv = (T*)A.dv + (long long)b * A.dvs[0] + (long long)key * A.dvs[1] + (long long)hk * A.dvs[2];
@@ -349,11 +448,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xattn_dkv_kernel(XaArgs
   }
 }
 
-// adds the shares up: out[b][l][head in group][d] over rows = G * L of each of the B * Hkv heads, 8 channels per thread
+// adds the shares up (dq, or dk and dv by blockIdx.y): out[b][l][head in group][d] over rows = G * L of each of the B * Hkv heads, 8 channels per thread
+struct XaSum { void* out; long long sb, sl, sh; };
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_sum_kernel(const float* __restrict__ part, int nsplit, int heads, int Hkv, int G,
-                                                        int L, int D, T* __restrict__ out, long long sb, long long sl,
-                                                        long long sh) {
+                                                        int L, int D, XaSum first, XaSum second) {
+  const XaSum S = blockIdx.y ? second : first;
+  part += (long long)blockIdx.y * nsplit * heads * G * L * D;
   const int chunks = D >> 3, rows = G * L;
   const long long all = (long long)heads * rows, i = blockIdx.x * 256ll + threadIdx.x;
   if (i >= all * chunks) return;
@@ -367,7 +468,7 @@ __global__ __launch_bounds__(256) void xattn_sum_kernel(const float* __restrict_
   }
   const int head = (int)(flat / rows), row = (int)(flat - (long long)head * rows);
   const int b = head / Hkv, hk = head % Hkv, g = row / L, l = row - g * L;
-  *reinterpret_cast<u32x4*>(out + b * sb + l * sl + (long long)(hk * G + g) * sh + d) =
+  *reinterpret_cast<u32x4*>((T*)S.out + b * S.sb + l * S.sl + (long long)(hk * G + g) * S.sh + d) =
       u32x4{xa_pack<T>(a[0], a[1]), xa_pack<T>(a[2], a[3]), xa_pack<T>(e[0], e[1]), xa_pack<T>(e[2], e[3])};
 }
 
@@ -388,8 +489,8 @@ static XaBwdPlan xa_bwd_plan(const ried_xattn_t& d) {
   };
   p.qtiles = ceil_div(rows, 128);
   p.qsplit = split(p.qtiles * heads, 512, d.keys / 256);
-  p.ktiles = ceil_div(d.keys, 128);
-  p.ksplit = split(p.ktiles * heads, d.dim <= 64 ? 512 : 256, rows / 256);
+  p.ktiles = ceil_div(d.keys, 64);
+  p.ksplit = split(p.ktiles * heads, XA_WANT_K, rows / 256);
   const long long a = p.qsplit > 1 ? p.qsplit * p.rows_all * d.dim : 0, b = p.ksplit > 1 ? 2 * p.ksplit * p.keys_all * d.dim : 0;
   p.floats = 2 * ((p.rows_all + 3) / 4 * 4) + (a > b ? a : b);
   return p;
@@ -405,7 +506,7 @@ extern "C" long long ried_xattn_bwd_scratch_floats(long long batch, long long qu
 
 template <typename T, int DP>
 static int xa_bwd_launch(XaArgs A, const XaBwdPlan& p, hipStream_t stream) {
-  constexpr int lq = 2 * 2 * 64 * XaTile<DP>::RB, lk = lq + 2 * 512;
+  constexpr int lq = 2 * 2 * 64 * XaTile<DP>::RB, lk = 2 * XaKv<DP>::STAGE;
   for (int i = 0; i < 2; ++i) {
     const hipError_t e = hipFuncSetAttribute(i ? (const void*)xattn_dkv_kernel<T, DP> : (const void*)xattn_dq_kernel<T, DP>,
                                              hipFuncAttributeMaxDynamicSharedMemorySize, i ? lk : lq);
@@ -417,18 +518,15 @@ static int xa_bwd_launch(XaArgs A, const XaBwdPlan& p, hipStream_t stream) {
   hipLaunchKernelGGL((xattn_dq_kernel<T, DP>), dim3((unsigned)(A.tiles * A.nsplit * heads)), dim3(256), lq, stream, A);
   if (A.nsplit > 1)
     hipLaunchKernelGGL((xattn_sum_kernel<T>), dim3(ceil_div(p.rows_all * (A.D >> 3), 256)), dim3(256), 0, stream, A.part,
-                       A.nsplit, heads, A.Hkv, A.G, A.Lq, A.D, (T*)A.dq, A.dqs[0], A.dqs[1], A.dqs[2]);
+                       A.nsplit, heads, A.Hkv, A.G, A.Lq, A.D, XaSum{A.dq, A.dqs[0], A.dqs[1], A.dqs[2]}, XaSum{});
   if (A.Lk == 0) return RIED_OK;
   A.tiles = p.ktiles;
   A.nsplit = p.ksplit;
-  hipLaunchKernelGGL((xattn_dkv_kernel<T, DP>), dim3((unsigned)(A.tiles * A.nsplit * heads)), dim3(256), lk, stream, A);
-  if (A.nsplit > 1) {
-    hipLaunchKernelGGL((xattn_sum_kernel<T>), dim3(ceil_div(p.keys_all * (A.D >> 3), 256)), dim3(256), 0, stream, A.part,
-                       A.nsplit, heads, A.Hkv, 1, A.Lk, A.D, (T*)A.dk, A.dks[0], A.dks[1], A.dks[2]);
-    hipLaunchKernelGGL((xattn_sum_kernel<T>), dim3(ceil_div(p.keys_all * (A.D >> 3), 256)), dim3(256), 0, stream,
-                       A.part + A.nsplit * p.keys_all * A.D, A.nsplit, heads, A.Hkv, 1, A.Lk, A.D, (T*)A.dv, A.dvs[0],
-                       A.dvs[1], A.dvs[2]);
-  }
+  hipLaunchKernelGGL((xattn_dkv_kernel<T, DP>), dim3((unsigned)(A.tiles * A.nsplit * heads)), dim3(64 * XaKv<DP>::NW), lk, stream, A);
+  if (A.nsplit > 1)
+    hipLaunchKernelGGL((xattn_sum_kernel<T>), dim3(ceil_div(p.keys_all * (A.D >> 3), 256), 2), dim3(256), 0, stream, A.part,
+                       A.nsplit, heads, A.Hkv, 1, A.Lk, A.D, XaSum{A.dk, A.dks[0], A.dks[1], A.dks[2]},
+                       XaSum{A.dv, A.dvs[0], A.dvs[1], A.dvs[2]});
   return RIED_OK;
 }
 template <typename T>

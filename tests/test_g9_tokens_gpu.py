@@ -342,6 +342,18 @@ def test_cross_attention_lengths_and_masks(shape, kind):
     assert torch.equal(attention.cross_attention(q.detach(), k, v, over), attention.cross_attention(q.detach(), k, v, like))
 
 
+@pytest.mark.parametrize("keys", [8192, 16384 + 100, 40000])
+def test_cross_attention_many_shares_of_the_keys(keys):
+    """One row over enough keys that they are shared out to up to 64 blocks, some of them without a key that counts."""
+    q, k, v = qkv(keys, 2, 1, keys, 4, 1, 64, BF16)
+    cross_check(q, k, v, train=False)
+    cross_check(q, k, v, torch.tensor([keys, 33], dtype=torch.int32, device=DEV), train=False)
+    mask = torch.zeros(2, keys, dtype=torch.bool, device=DEV)
+    mask[0, keys - 5:] = True
+    mask[1, ::97] = True
+    cross_check(q, k, v, None, mask, train=False)
+
+
 def test_cross_attention_no_keys_no_queries_no_batch():
     for B, Lq, Lk in ((2, 3, 0), (2, 0, 3), (0, 3, 3)):
         q, k, v = (t.requires_grad_() for t in qkv(1, B, Lq, Lk, 4, 2, 64, BF16))

@@ -6,21 +6,21 @@
 #include "xattn.h"
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Tiles: a block of four waves owns 128 rows, a wave 32; tiles of 64 keys go HBM -> LDS by DMA, two stages, one barrier
-// per tile.  S^T = K Q^T leaves a row's scores in one lane pair, so the softmax runs in registers, and P^T is the B operand
+// Tiles: a wave owns 32 rows, a block of NW waves 32 NW; tiles of 64 keys go HBM -> LDS by DMA, one barrier per tile.  S^T = K Q^T leaves a row's scores in one lane pair, so the softmax runs in registers, and P^T is the B operand
 // of O^T += V^T P^T as it stands.  The running maximum is raised only when a score exceeds it by more than 2^8 (the
 // sums hold that in fp32): rescaling is rare after the first tile.
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaArgs A) {
+template <int DP, int NW> struct XaFwd { static constexpr int STAGES = NW == 8 ? 3 : 2, LDS = STAGES * 2 * 64 * XaTile<DP>::RB; };
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void xattn_fwd_kernel(XaArgs A) {
   constexpr int KS = XaTile<DP>::KS, DT = XaTile<DP>::DT, RB = XaTile<DP>::RB, NC = XaTile<DP>::NC, RPI = XaTile<DP>::RPI;
-  constexpr int TILE = 64 * RB, NI = 16 / RPI;                    // DMA instructions per wave and operand
-  extern __shared__ __align__(16) char smem[];                    // [2][K tile, V tile]
+  constexpr int TILE = 64 * RB, NI = 64 / NW / RPI, NST = XaFwd<DP, NW>::STAGES;   // NI: DMA instructions per wave and operand
+  extern __shared__ __align__(16) char smem[];                    // [NST][K tile, V tile]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   int inner, head;
   xa_block(A.tiles * A.nsplit, A.B * A.Hkv, inner, head);
   const int b = head / A.Hkv, hk = head % A.Hkv, tile = inner % A.tiles, split = inner / A.tiles;
-  const int row = tile * 128 + wave * 32 + (lane & 31);
+  const int row = tile * (32 * NW) + wave * 32 + (lane & 31);
   const bool live = row < A.rows;
   const int g = live ? row / A.Lq : 0, qi = live ? row - g * A.Lq : 0;
   const T* qp = (const T*)A.q + (long long)b * A.qs[0] + (long long)qi * A.qs[1] + (long long)(hk * A.G + g) * A.qs[2];
@@ -44,9 +44,9 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaArgs A) {
     char* dst = smem + buf * 2 * TILE + wave * RPI * RB;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const unsigned bad = (w >> (srow + i * 4 * RPI)) & 1 ? 0u : XA_OOB;
-      xa_dma16(rk, koff | bad, i * 4 * RPI * krow, dst + i * 4 * RPI * RB);
-      xa_dma16(rv, voff | bad, i * 4 * RPI * vrow, dst + TILE + i * 4 * RPI * RB);
+      const unsigned bad = (w >> (srow + i * NW * RPI)) & 1 ? 0u : XA_OOB;
+      xa_dma16(rk, koff | bad, i * NW * RPI * krow, dst + i * NW * RPI * RB);
+      xa_dma16(rv, voff | bad, i * NW * RPI * vrow, dst + TILE + i * NW * RPI * RB);
     }
   };
   auto mask_byte = [&](int t) -> int {
@@ -59,22 +59,24 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaArgs A) {
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = xa_zero();
   XaTr<DP> tr(smem + TILE, lane);
-  u64 w = 0;
+  // Tiles are asked for NST - 1 ahead; past the end the DMA writes zeros, so that the counted wait holds.
+  u64 w[NST] = {};
   int byte = 0, buf = 0;
-  if (t0 < t1) {
-    w = xa_word(nk - t0 * 64, mp != nullptr, mask_byte(t0));
-    issue(t0, w, 0);
-    byte = mask_byte(t0 + 1);
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i) {
+    w[i] = t0 + i < t1 ? xa_word(nk - (t0 + i) * 64, mp != nullptr, mask_byte(t0 + i)) : 0;
+    if (t0 < t1) issue(t0 + i < t1 ? t0 + i : t0, w[i], i);
   }
+  if (t0 < t1) byte = mask_byte(t0 + NST - 1);
   for (int t = t0; t < t1; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();                                 // tile t has landed; everyone is done with the other stage
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * 2 * NI) : "memory");
+    __builtin_amdgcn_s_barrier();                                 // tile t has landed; everyone is done with the tile before it
     asm volatile("" ::: "memory");
-    u64 wn = 0;
-    if (t + 1 < t1) {
-      wn = xa_word(nk - (t + 1) * 64, mp != nullptr, byte);
-      issue(t + 1, wn, buf ^ 1);
-      byte = mask_byte(t + 2);
+    {
+      const int n = t + NST - 1;
+      w[NST - 1] = n < t1 ? xa_word(nk - n * 64, mp != nullptr, byte) : 0;
+      byte = mask_byte(n + 1);
+      issue(n < t1 ? n : t0, w[NST - 1], buf == 0 ? NST - 1 : buf - 1);
     }
     {
       const char* kt = smem + buf * 2 * TILE;
@@ -85,10 +87,10 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaArgs A) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) s[u] = xa_mma<T>(xa_frag<DP>(kt, 32 * u, ks, lane), fq[ks], s[u]);
       
-      if (w != ~0ull) {
+      if (w[0] != ~0ull) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const unsigned bits = (unsigned)(w >> (32 * u)) >> (4 * h);
+          const unsigned bits = (unsigned)(w[0] >> (32 * u)) >> (4 * h);
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[u][r] = (bits >> (8 * (r >> 2) + (r & 3))) & 1 ? s[u][r] : -INFINITY;
         }
@@ -129,10 +131,12 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaArgs A) {
       add(XaInt<0>{}), add(XaInt<1>{}), add(XaInt<2>{}), add(XaInt<3>{});
       
     }
-    w = wn;
-    tr.move(buf ? -2 * TILE : 2 * TILE);
-    buf ^= 1;
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i) w[i] = w[i + 1];
+    tr.move(buf == NST - 1 ? -(NST - 1) * 2 * TILE : 2 * TILE);
+    buf = buf == NST - 1 ? 0 : buf + 1;
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                // no DMA may outlive the block
   float lo, hi;
   xa_halves(sum, lo, hi);
   const float total = lo + hi;
@@ -388,13 +392,18 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs A) {
 // ---------------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------------
-struct XaSplit { int tiles, nsplit; };
+#ifndef XA_NW8
+#define XA_NW8 1
+#endif
+struct XaSplit { int tiles, nsplit, nw; };
 // Shares of the keys per block row: the forward kernels want 512 blocks (two per CU, one for single tokens at D > 64);
 // a share keeps at least 4 tiles per wave that reads it.
 static XaSplit xa_fwd_split(const ried_xattn_t& d) {
   const long long rows = d.heads / d.groups * d.queries, heads = d.batch * d.groups;
   XaSplit s;
-  s.tiles = rows <= 32 ? 1 : ceil_div(rows, 128);
+  // eight waves where 256 rows a block still give every CU one
+  s.nw = XA_NW8 && rows > 128 && ceil_div(rows, 256) * heads >= 256 ? 8 : 4;
+  s.tiles = rows <= 32 ? 1 : ceil_div(rows, 32 * s.nw);
   const long long blocks = s.tiles * heads;
   const long long want = rows <= 32 && d.dim > 64 ? 256 : 512, most = rows <= 32 ? d.keys / 512 : d.keys / 256;
   long long n = want / (blocks > 0 ? blocks : 1);
@@ -467,9 +476,14 @@ static int xa_fwd_launch(const XaArgs& A, hipStream_t stream) {
     if (int e = xa_lds(xattn_token_kernel<T, DP>, lds, "ried_xattn_fwd")) return e;
     hipLaunchKernelGGL((xattn_token_kernel<T, DP>), dim3(grid), dim3(256), lds, stream, A);
   } else {
-    constexpr int lds = 2 * 2 * 64 * XaTile<DP>::RB;
-    if (int e = xa_lds(xattn_fwd_kernel<T, DP>, lds, "ried_xattn_fwd")) return e;
-    hipLaunchKernelGGL((xattn_fwd_kernel<T, DP>), dim3(grid), dim3(256), lds, stream, A);
+    constexpr int lds4 = XaFwd<DP, 4>::LDS, lds8 = XaFwd<DP, 8>::LDS;
+    if (A.nw == 8) {
+      if (int e = xa_lds(xattn_fwd_kernel<T, DP, 8>, lds8, "ried_xattn_fwd")) return e;
+      hipLaunchKernelGGL((xattn_fwd_kernel<T, DP, 8>), dim3(grid), dim3(512), lds8, stream, A);
+    } else {
+      if (int e = xa_lds(xattn_fwd_kernel<T, DP, 4>, lds4, "ried_xattn_fwd")) return e;
+      hipLaunchKernelGGL((xattn_fwd_kernel<T, DP, 4>), dim3(grid), dim3(256), lds4, stream, A);
+    }
   }
   if (A.nsplit > 1)
     hipLaunchKernelGGL((xattn_join_kernel<T>), dim3(ceil_div((long long)A.B * A.Hkv * A.rows, 4)), dim3(256), 0, stream, A);
@@ -489,6 +503,7 @@ extern "C" int ried_xattn_fwd(const ried_xattn_t* desc, hipStream_t stream) {
   const XaSplit s = xa_fwd_split(d);
   A.tiles = s.tiles;
   A.nsplit = s.nsplit;
+  A.nw = s.nw;
   RIED_CHECK_ARG((long long)A.tiles * A.nsplit * A.B * A.Hkv <= 0x7fffffffll, "ried_xattn_fwd: too many blocks");
   if (A.nsplit > 1) {
     RIED_CHECK_ARG(d.scratch, "ried_xattn_fwd: this call needs ried_xattn_fwd_scratch_floats() of scratch");

@@ -6,6 +6,7 @@ tensors, as on the drop-in module route; the fused TrainStep has its own update 
 from __future__ import annotations
 
 from array import array
+from operator import attrgetter
 from typing import Dict, List
 
 import torch
@@ -19,6 +20,10 @@ BLOCK = 256           # elements that share a scale of the 8-bit moments; every 
 CHUNK = 4096          # elements per workgroup
 CODES = torch.float8_e4m3fn
 
+# (applied to all of a group's tensors by map: a Python loop over a few hundred tensors takes longer than their update)
+_grad, _dtype = attrgetter("grad"), attrgetter("dtype")
+_address, _elements, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+
 
 class _Bank:
     """The tensors of one group that share an element type: their moments in flat buffers, the kernel's job table."""
@@ -26,6 +31,7 @@ class _Bank:
     def __init__(self, params: List[torch.Tensor], bits: int):
         self.params, self.bits = params, bits
         self.dtype, self.device = params[0].dtype, params[0].device
+        self.kinds = {self.dtype}
         self.sizes = [p.numel() for p in params]
         self.starts, blocks, first, pairs = [], 0, [0], []
         for i, n in enumerate(self.sizes):
@@ -69,13 +75,37 @@ class _Bank:
             _check_param(p)
             if p.numel() != n or p.dtype is not self.dtype or p.device != self.device:
                 raise RuntimeError("AdamW: a parameter changed its size, type or device after the optimizer's first step")
-        one = 4 if self.bits == 32 else 1
+        one = 4 if self.bits == 32 else 1                     # bytes of a moment
         m, v = (self.flat[k].data_ptr() for k in self.flat if not k.endswith("_scale"))
         ms, vs = (self.flat[k].data_ptr() for k in self.flat if k.endswith("_scale")) if self.bits == 8 else (0, 0)
         rows = [(p, m + s * one, v + s * one, ms and ms + s // BLOCK * 4, vs and vs + s // BLOCK * 4, n)
                 for p, s, n in zip(at, self.starts, self.sizes)]
         self.tables.append(torch.tensor(rows, dtype=torch.int64).to(self.device))
         self.at = at
+
+
+    def gradients(self):
+        """Addresses of the gradients (0: none), and the copies that stand in for those that are not contiguous."""
+        grads = list(map(_grad, self.params))
+        try:
+            if list(map(_elements, grads)) == self.sizes and set(map(_dtype, grads)) == self.kinds and all(map(_contiguous, grads)):
+                return array("q", map(_address, grads)), ()
+        except (TypeError, AttributeError, RuntimeError):     # a tensor without a gradient, a sparse one
+            pass
+        at, kept = array("q"), []
+        for p, n, g in zip(self.params, self.sizes, grads):
+            if g is None:
+                at.append(0)
+                continue
+            if g.dtype is not self.dtype or g.layout is not torch.strided:
+                raise TypeError(f"AdamW: gradients are dense and of their parameter's type, not {g.layout} {g.dtype}")
+            if g.numel() != n:
+                raise ValueError(f"AdamW: a gradient of {g.numel()} elements for a parameter of {n}")
+            if not g.is_contiguous():
+                g = g.contiguous()
+                kept.append(g)
+            at.append(g.data_ptr())
+        return at, kept
 
 
 def _check_param(p: torch.Tensor):
@@ -193,21 +223,10 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         for gi, group in enumerate(self.param_groups):
             for bank in self._group_banks(gi, group):
-                at = [p.data_ptr() for p in bank.params]
+                at = list(map(_address, bank.params))
                 if at != bank.at:
                     bank.bind(at)
-                grads, kept = array("q"), []
-                for p in bank.params:
-                    g = p.grad
-                    if g is None:
-                        grads.append(0)
-                        continue
-                    if g.dtype is not bank.dtype or g.layout is not torch.strided:
-                        raise TypeError(f"AdamW: gradients are dense and of their parameter's type, not {g.layout} {g.dtype}")
-                    if not g.is_contiguous():
-                        g = g.contiguous()
-                        kept.append(g)
-                    grads.append(g.data_ptr())
+                grads, kept = bank.gradients()
                 ops.adamw_jobs(bank.tables[-1], bank.map, grads, bank.first, bank.steps, bank.coef, float(group["lr"]),
                                group["betas"][0], group["betas"][1], group["eps"], group["weight_decay"], bank.dtype, bank.bits)
         return loss

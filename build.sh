@@ -22,6 +22,16 @@ for f in api gemm elementwise special ssim loader legacy attn norm rotary xattn 
   fi
   objs+=($f.o)
 done
+# the direct calls of the token operators (host code: torch tensors and autograd nodes in front of the C ABI)
+if [ ! -f ../_bind.so ] || [ bind.cpp -nt ../_bind.so ] || [ ../../include/ried_gan.h -nt ../_bind.so ]; then
+  echo "g++ bind.cpp"
+  rm -f ../_bind.so
+  T=$(python3 -c "import os, torch; print(os.path.dirname(torch.__file__))")
+  PY=$(python3 -c "import sysconfig; print(sysconfig.get_paths()['include'])")
+  g++ -O2 -std=c++17 -fPIC -shared -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM=1 -I$T/include -I$T/include/torch/csrc/api/include \
+    -I$PY -I/opt/rocm/include bind.cpp -o ../_bind.so -L$T/lib -lc10 -lc10_hip -ltorch_cpu -ltorch_python &
+  pids+=($!)
+fi
 for p in "${pids[@]}"; do wait $p; done
 hipcc --offload-arch=gfx950 -shared -fPIC -o $OUT "${objs[@]}"
 echo "built $OUT"

@@ -116,3 +116,19 @@ class _Lib:
 
 
 lib = _Lib()
+_direct = None
+
+
+def direct():
+    """The module of direct calls (csrc/bind.cpp), connected to the loaded library."""
+    global _direct
+    if _direct is None:
+        dll = lib.load()
+        try:
+            import torch  # noqa: F401  (first: the module's symbols are torch's)
+            from . import _bind
+        except ImportError as e:
+            raise RuntimeError(f"reid_gan_amd/_bind.so does not load: build it with ./build.sh ({e})") from e
+        _bind.connect({name: ctypes.cast(getattr(dll, name), ctypes.c_void_p).value for name in lib.protos})
+        _direct = _bind
+    return _direct

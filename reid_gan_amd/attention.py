@@ -1,6 +1,9 @@
 """Token operators of a cross-attention block, beside the convolutional path: layer norm, rotary positions of several
 axes, and cross attention to an encoder's states, forward and backward on hand-written kernels.
 
+A call whose arguments need nothing but the launch goes straight to it (csrc/bind.cpp); the Python code here does the rest:
+the checks with their messages, and the copies of what is not laid out for the kernels.
+
 They have no counterpart in the reference, whose only attention is the Self_Attn layer (src/rinet.py:150-181).
 Tensors live on a ROCm device (there is no CPU path) in fp32, bf16 or fp16 (cross attention: bf16 or fp16); sums,
 statistics and softmax are fp32 whatever the type.  Every call runs on the current stream of its tensors' device and
@@ -19,6 +22,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import ops
+from ._lib import direct
 
 __all__ = ["layer_norm", "LayerNorm", "rotary", "rotary_frequencies", "cross_attention"]
 
@@ -123,6 +127,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     x: any shape; rows are read where they lie when their channels are adjacent.  weight, bias: [C], contiguous, both fp32
     or both of x's type, each optional.  The result is contiguous and of x's type; weight and bias gradients are summed
     in fp32 in a fixed order."""
+    y = direct().layer_norm(x, weight, bias, eps)
+    if y is not None:
+        return y
     _check_layer_norm(x, weight, bias, eps)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
@@ -198,6 +205,10 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sectio
     rotary_frequencies, sum(sections) entries.  Pair j is channels (j, j + pairs), or (2j, 2j + 1) when interleaved;
     channels behind the pairs pass through.  Angles are formed in 64 bits, so far positions keep their precision.
     inverse turns back (and is the gradient).  out: where to write, also x itself (no gradients then)."""
+    if out is None:
+        y = direct().rotary(x, positions, freqs, sections, interleaved, inverse)
+        if y is not None:
+            return y
     _check_tensor("rotary", "x", x, ops.TOKEN_TYPES)
     if x.dim() != 4:
         raise ValueError("rotary: x is [batch][tokens][heads][channels]")
@@ -295,6 +306,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: 
     keys gives zeros and no gradient; hidden keys have no effect whatever they hold, and get zero gradients.  scale:
     channels ** -0.5 unless given.  channels: a multiple of 8 up to 128, bf16 or fp16.  Views are read where they lie when
     their channels are adjacent and their strides are multiples of 8 elements; others are copied."""
+    o = direct().cross_attention(q, k, v, lengths, key_mask, scale)
+    if o is not None:
+        return o
     _check_tensor("cross_attention", "q", q, _CROSS_TYPES)
     device, kind = q.device, (q.dtype,)
     _check_tensor("cross_attention", "k", k, kind, device)

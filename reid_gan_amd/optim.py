@@ -6,12 +6,12 @@ tensors, as on the drop-in module route; the fused TrainStep has its own update 
 from __future__ import annotations
 
 from array import array
-from operator import attrgetter
 from typing import Dict, List
 
 import torch
 
 from . import ops
+from ._lib import direct
 
 __all__ = ["AdamW"]
 
@@ -20,10 +20,6 @@ BLOCK = 256           # elements that share a scale of the 8-bit moments; every 
 CHUNK = 4096          # elements per workgroup
 CODES = torch.float8_e4m3fn
 
-# (applied to all of a group's tensors by map: a Python loop over a few hundred tensors takes longer than their update)
-_grad, _dtype = attrgetter("grad"), attrgetter("dtype")
-_address, _elements, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
-
 
 class _Bank:
     """The tensors of one group that share an element type: their moments in flat buffers, the kernel's job table."""
@@ -31,7 +27,6 @@ class _Bank:
     def __init__(self, params: List[torch.Tensor], bits: int):
         self.params, self.bits = params, bits
         self.dtype, self.device = params[0].dtype, params[0].device
-        self.kinds = {self.dtype}
         self.sizes = [p.numel() for p in params]
         self.starts, blocks, first, pairs = [], 0, [0], []
         for i, n in enumerate(self.sizes):
@@ -54,7 +49,9 @@ class _Bank:
                     self.flat[name] = torch.zeros(many, dtype=torch.uint8, device=self.device).view(CODES)
                     self.flat[name + "_scale"] = torch.zeros(many // BLOCK, dtype=F32, device=self.device)
         self.tables: List[torch.Tensor] = []          # (earlier ones stay: a captured graph may hold their address)
-        self.at: List[int] = []
+        self.at = array("q")
+        self.elements = array("q", self.sizes)
+        self.grads = array("q", bytes(8 * len(params)))
 
     def views(self, i: int) -> Dict[str, torch.Tensor]:
         """The state of tensor i, as views of the flat buffers."""
@@ -67,7 +64,7 @@ class _Bank:
                 out[name] = buf[start:start + n].view(shape)
         return out
 
-    def bind(self, at: List[int]):
+    def bind(self, at):
         """Build the job table for parameters at these addresses."""
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: the parameters moved (or this is the first step); run a step before the capture")
@@ -85,27 +82,28 @@ class _Bank:
 
 
     def gradients(self):
-        """Addresses of the gradients (0: none), and the copies that stand in for those that are not contiguous."""
-        grads = list(map(_grad, self.params))
-        try:
-            if list(map(_elements, grads)) == self.sizes and set(map(_dtype, grads)) == self.kinds and all(map(_contiguous, grads)):
-                return array("q", map(_address, grads)), ()
-        except (TypeError, AttributeError, RuntimeError):     # a tensor without a gradient, a sparse one
-            pass
-        at, kept = array("q"), []
-        for p, n, g in zip(self.params, self.sizes, grads):
+        """Addresses of the gradients in self.grads (0: none); returns the copies that stand in for those that are not
+        contiguous.  Follows parameters that moved."""
+        if direct().gradients(self.params, self.at, self.elements, self.grads):
+            return ()
+        at = array("q", [p.data_ptr() for p in self.params])
+        if at != self.at:
+            self.bind(at)
+        kept = []
+        for i, (p, n) in enumerate(zip(self.params, self.sizes)):
+            g = p.grad
             if g is None:
-                at.append(0)
+                self.grads[i] = 0
                 continue
             if g.dtype is not self.dtype or g.layout is not torch.strided:
                 raise TypeError(f"AdamW: gradients are dense and of their parameter's type, not {g.layout} {g.dtype}")
-            if g.numel() != n:
-                raise ValueError(f"AdamW: a gradient of {g.numel()} elements for a parameter of {n}")
+            if g.numel() != n or g.device != self.device:
+                raise ValueError(f"AdamW: a gradient of {g.numel()} elements on {g.device} for a parameter of {n} on {self.device}")
             if not g.is_contiguous():
                 g = g.contiguous()
                 kept.append(g)
-            at.append(g.data_ptr())
-        return at, kept
+            self.grads[i] = g.data_ptr()
+        return kept
 
 
 def _check_param(p: torch.Tensor):
@@ -223,10 +221,7 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         for gi, group in enumerate(self.param_groups):
             for bank in self._group_banks(gi, group):
-                at = list(map(_address, bank.params))
-                if at != bank.at:
-                    bank.bind(at)
-                grads, kept = bank.gradients()
-                ops.adamw_jobs(bank.tables[-1], bank.map, grads, bank.first, bank.steps, bank.coef, float(group["lr"]),
+                kept = bank.gradients()                            # noqa: F841  (alive until the launch)
+                ops.adamw_jobs(bank.tables[-1], bank.map, bank.grads, bank.first, bank.steps, bank.coef, float(group["lr"]),
                                group["betas"][0], group["betas"][1], group["eps"], group["weight_decay"], bank.dtype, bank.bits)
         return loss

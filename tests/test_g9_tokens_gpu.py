@@ -488,6 +488,43 @@ def test_cross_attention_is_the_same_every_time():
 
 
 # --------------------------------------------------------------------------- streams, graphs, threads
+class Sub(torch.Tensor):
+    """A subclass keeps a call from going straight to the kernels: the checks and copies in Python see it."""
+
+
+@pytest.mark.parametrize("plain", [True, False])
+def test_calls_and_gradients_by_both_ways(plain):
+    """The direct calls and the Python functions behind them give the same bits; neither has a second derivative."""
+    g = gen(90)
+    as_ = (lambda t: t) if plain else (lambda t: t.as_subclass(Sub))
+    bare = lambda t: t.as_subclass(torch.Tensor)
+    x, w, b, dy = normal(g, 40, 96, to=BF16), normal(g, 96), normal(g, 96), normal(g, 40, 96, to=BF16)
+    r, pos, sections = normal(g, 2, 7, 4, 64, to=BF16), torch.randint(0, 99, (2, 7, 3), generator=g, device=DEV), (8, 12, 12)
+    freqs = attention.rotary_frequencies(sections)
+    q, k, v = qkv(91, 2, 50, 70, 4, 2, 64, BF16)
+    d = normal(g, 2, 50, 4, 64, to=BF16)
+    mask = torch.rand(2, 70, generator=g, device=DEV) < 0.5
+    calls = [(lambda *t: attention.layer_norm(*t), (x, w, b), dy), (lambda t: attention.rotary(t, pos, freqs, sections), (r,), r.clone()),
+             (lambda *t: attention.cross_attention(*t, key_mask=mask), (q, k, v), d)]
+    for call, inputs, grad in calls:
+        stats = []
+        for other in (False, True):
+            leaves = [(t if other else as_(t)).detach().clone().requires_grad_() for t in inputs]
+            out = call(*leaves)
+            grads = torch.autograd.grad(out, leaves, grad, retain_graph=True)
+            with torch.no_grad():
+                again = call(*leaves)
+            assert torch.equal(bare(out.detach()), bare(again))
+            stats.append([bare(out.detach()), *(bare(t) for t in grads)])
+            some = torch.autograd.grad(out, leaves[:1], grad)                       # only one of the gradients
+            assert torch.equal(bare(some[0]), stats[-1][1])
+        assert all(torch.equal(a, c) for a, c in zip(*stats))
+        leaves = [as_(t).detach().clone().requires_grad_() for t in inputs]
+        first = torch.autograd.grad(call(*leaves), leaves, grad.detach().clone().requires_grad_(), create_graph=True)
+        with pytest.raises(RuntimeError, match="twice"):
+            first[0].float().sum().backward()
+
+
 def test_two_streams_at_once():
     sets = [qkv(20 + i, 2, 1, 2000, 8, 2, 128, BF16) for i in range(2)]
     want = [attention.cross_attention(*s) for s in sets]

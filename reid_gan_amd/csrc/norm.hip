@@ -288,22 +288,23 @@ __global__ __launch_bounds__(256) void ln_dw_wide_kernel(const T* __restrict__ d
   part[(long long)blockIdx.y * 2 * C + C + c] = ab;
 }
 
-// dw, db = sums of the partial rows: 32 columns by 8 slices of the rows per block, the slices joined in LDS
+// dw, db = sums of the partial rows: 32 columns by 32 slices of the rows per block, the slices joined in LDS
 template <typename W>
-__global__ __launch_bounds__(256) void ln_finish_kernel(const float* __restrict__ part, int nparts, int C,
-                                                        W* __restrict__ dw, W* __restrict__ db) {
-  __shared__ float sh[8][33];
+__global__ __launch_bounds__(1024) void ln_finish_kernel(const float* __restrict__ part, int nparts, int C,
+                                                         W* __restrict__ dw, W* __restrict__ db) {
+  __shared__ float sh[32][33];
   const int lc = threadIdx.x & 31, q = threadIdx.x >> 5, c = blockIdx.x * 32 + lc;   // c over [dw | db]
   float s = 0.f;
   if (c < 2 * C) {
 #pragma unroll 8
-    for (int r = q; r < nparts; r += 8) s += part[(long long)r * 2 * C + c];
+    for (int r = q; r < nparts; r += 32) s += part[(long long)r * 2 * C + c];
   }
   sh[q][lc] = s;
   __syncthreads();
   if (q == 0 && c < 2 * C) {
+    s = 0.f;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += sh[i][lc];
+    for (int i = 0; i < 32; ++i) s += sh[i][lc];
     if (c < C) {
       if (dw) dw[c] = TokType<W>::down(s);
     } else if (db) {
@@ -312,7 +313,9 @@ __global__ __launch_bounds__(256) void ln_finish_kernel(const float* __restrict_
   }
 }
 
-#define LN_MAX_PARTS 512
+// blocks of the backward kernel, each of which leaves a partial row: what the registers let the chip hold (16 waves per CU
+// up to two chunks per lane, 8 above)
+#define LN_MAX_PARTS(nv) ((nv) == 1 || (nv) == 2 ? 1024 : 512)
 // rows a block of the backward kernel takes at a time, and whether the register kernels hold the row
 struct LnPlan { int nv, lpr, wpr; };
 static LnPlan ln_plan(int type, int C) {
@@ -343,7 +346,8 @@ static int ln_parts(long long rows, int type, int C) {
   const LnPlan pl = ln_plan(type, C);
   const long long per = pl.nv == 0 ? 64 : pl.wpr > 1 ? 1 : 256 / pl.lpr;
   long long n = (rows + per - 1) / per;
-  return (int)(n > LN_MAX_PARTS ? LN_MAX_PARTS : n);
+  const int most = pl.wpr > 1 ? LN_MAX_PARTS(pl.nv) / pl.wpr * 2 : LN_MAX_PARTS(pl.nv);
+  return (int)(n > most ? most : n);
 }
 
 extern "C" long long ried_layer_norm_bwd_scratch_floats(long long rows, int C, int type) {
@@ -412,7 +416,7 @@ extern "C" int ried_layer_norm_bwd(const void* dy, long long lddy, const void* x
     });
   }
   if (sums) {                                                      // (no rows: the sums are zeros)
-    TOK_DISPATCH(wtype, W, hipLaunchKernelGGL((ln_finish_kernel<W>), dim3(ceil_div(2ll * C, 32)), dim3(256), 0, stream,
+    TOK_DISPATCH(wtype, W, hipLaunchKernelGGL((ln_finish_kernel<W>), dim3(ceil_div(2ll * C, 32)), dim3(1024), 0, stream,
                                               scratch, nparts, C, (W*)dw, (W*)db));
   }
   RIED_CHECK_LAUNCH("ried_layer_norm_bwd");

@@ -179,8 +179,10 @@ struct XaArgs {
   float scale;
 };
 
-// the block's share of the grid: blockIdx.x runs over (tile, split) of a (batch, key head); when the heads divide into
-// whole rounds of the 8 XCDs, all blocks of a head run on one XCD, so its keys and values are fetched into one L2
+// The block's share of the grid: blockIdx.x runs over (tile, split) of a (batch, key head).  Workgroups go to the 8 XCDs in
+// turn; when the heads divide into whole rounds of 8, all blocks of a head run on one XCD, so that its keys and values are
+// fetched into one L2.  (Dealing a head's blocks out to all XCDs where lengths are ragged evens their work out, and
+// measured the same.)
 __device__ __forceinline__ void xa_block(int per_head, int heads, int& inner, int& head) {
   const int id = blockIdx.x;
   if ((heads & 7) == 0) {

@@ -392,20 +392,20 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs A) {
 // ---------------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------------
-#ifndef XA_NW8
-#define XA_NW8 1
-#endif
 struct XaSplit { int tiles, nsplit, nw; };
-// Shares of the keys per block row: the forward kernels want 512 blocks (two per CU, one for single tokens at D > 64);
-// a share keeps at least 4 tiles per wave that reads it.
+// Waves a block, row tiles and shares of the keys.  Where blocks of eight waves (256 rows) give every CU one, they are taken -
+// half the DMA a row - and the keys stay whole; with ragged lengths only where there are several per CU, because blocks
+// then differ (4 x 4096 rows over 657 to 1500 keys: 35 us with four waves, 39 with eight).  Otherwise four waves, and the
+// keys are shared out until there are 512 blocks (256 for single tokens at D > 64, one per CU), a share keeping at least
+// four tiles per wave that reads it.  The shares do not depend on `lengths`: the scratch size has to be known without.
 static XaSplit xa_fwd_split(const ried_xattn_t& d) {
-  const long long rows = d.heads / d.groups * d.queries, heads = d.batch * d.groups;
+  const long long rows = d.heads / d.groups * d.queries, heads = d.batch * d.groups, wide = ceil_div(rows, 256) * heads;
   XaSplit s;
-  // eight waves where 256 rows a block still give every CU one
-  s.nw = XA_NW8 && rows > 128 && ceil_div(rows, 256) * heads >= 256 ? 8 : 4;
+  s.nw = rows > 128 && wide >= (d.lengths ? 1024 : 256) ? 8 : 4;
   s.tiles = rows <= 32 ? 1 : ceil_div(rows, 32 * s.nw);
-  const long long blocks = s.tiles * heads;
-  const long long want = rows <= 32 && d.dim > 64 ? 256 : 512, most = rows <= 32 ? d.keys / 512 : d.keys / 256;
+  s.nsplit = 1;
+  if (rows > 128 && wide >= 256) return s;
+  const long long blocks = s.tiles * heads, want = rows <= 32 && d.dim > 64 ? 256 : 512, most = rows <= 32 ? d.keys / 512 : d.keys / 256;
   long long n = want / (blocks > 0 ? blocks : 1);
   if (n > most) n = most;
   if (n > 64) n = 64;

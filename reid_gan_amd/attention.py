@@ -38,6 +38,8 @@ def _check_tensor(what: str, name: str, t, types, device=None):
         raise TypeError(f"{what}: {name} is {t.dtype}, not one of {', '.join(str(d).replace('torch.', '') for d in types)}")
     if device is not None and t.device != device:
         raise ValueError(f"{what}: {name} is on {t.device}, not on {device}")
+    if t.layout is not torch.strided or t.is_neg():
+        raise ValueError(f"{what}: {name} is sparse or a lazily negated view; pass a dense tensor (resolve_neg())")
 
 
 def _on_gpu(what: str, t: torch.Tensor):
@@ -248,6 +250,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sectio
         _on_gpu("rotary", x)
         if not adjacent:
             x = x.contiguous()
+        torch.autograd.graph.increment_version(out)              # (a graph that saved what is written here must not use it)
     ops.rotary(x, out, positions, freqs, sections, interleaved, inverse)
     return out
 

@@ -230,7 +230,7 @@ bool take(PyObject* o, Tensor& t, bool optional = false) {
   if (optional && o == Py_None) return true;
   if (!THPVariable_CheckExact(o)) return false;
   t = THPVariable_Unpack(o);
-  return t.layout() == at::kStrided;
+  return t.layout() == at::kStrided && !t.is_neg();
 }
 bool number(PyObject* o, double& v) {
   if (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o)) return false;
@@ -353,6 +353,7 @@ struct Words {
 
 // gradients(params, addresses, sizes, out): out[i] = address of the i-th parameter's gradient (0: none).  False when a
 // parameter is not at its address any more, or a gradient is not a contiguous one of the parameter's type and size.
+// Parameters with a gradient count as written (an earlier graph that saved one must not use it any more).
 PyObject* py_gradients(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 4 || !PyList_CheckExact(a[0])) Py_RETURN_FALSE;
@@ -370,10 +371,12 @@ PyObject* py_gradients(PyObject*, PyObject* const* a, Py_ssize_t n) {
       continue;
     }
     if (g.layout() != at::kStrided || g.scalar_type() != p.scalar_type() || g.numel() != sizes.data()[i] || g.device() != p.device() ||
-        !g.is_contiguous())
+        !g.is_contiguous() || g.is_neg())
       Py_RETURN_FALSE;
     out.data()[i] = reinterpret_cast<int64_t>(g.const_data_ptr());
   }
+  for (Py_ssize_t i = 0; i < many; ++i)
+    if (out.data()[i]) torch::autograd::impl::bump_version(THPVariable_Unpack(PyList_GET_ITEM(a[0], i)));
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }

@@ -126,9 +126,10 @@ __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void ln_bwd_kernel(
     for (int j = 0; j < NV; ++j) {
       tok_up(rx[j], xh[j]);
       tok_up(rg[j], g[j]);
+      const int n = C - (j * GS + l) * V;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        xh[j][i] = (xh[j][i] - mu) * rs;                          // (past the end: dy is 0 there)
+        xh[j][i] = i < n ? (xh[j][i] - mu) * rs : 0.f;            // (past the end dy is 0, but mu rs may be infinite)
         aw[j][i] += g[j][i] * xh[j][i];
         ab[j][i] += g[j][i];
         g[j][i] *= wv[j][i];
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(1024) void ln_bwd_wide_kernel(const T* __restrict__
     if (w) tok_load_n<W, V>(w + c, C - c, t);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      f[i] = (f[i] - mu) * rs;
+      f[i] = c + i < C ? (f[i] - mu) * rs : 0.f;
       if (w) g[i] *= t[i];
     }
   };
@@ -365,7 +366,8 @@ extern "C" long long ried_layer_norm_bwd_scratch_floats(long long rows, int C, i
   RIED_CHECK_ARG(rows >= 0 && C > 0 && C <= (1 << 24), name ": bad sizes (%lld rows of %d)", rows, C);               \
   RIED_CHECK_ARG(tok_type_ok(type) && (wtype == RIED_T_F32 || wtype == type),                                        \
                  name ": types are 0 fp32, 1 bf16, 2 fp16; parameters are fp32 or of the rows' type");               \
-  RIED_CHECK_ARG(rows <= 0x7fffffffll, name ": more than 2^31 - 1 rows")
+  const LnPlan pl = ln_plan(type, C);                                                                                 \
+  RIED_CHECK_ARG(rows < (1ll << 32) / (pl.nv == 0 ? 1024 : pl.lpr * pl.wpr) - 256, name ": too many rows (%lld)", rows)
 
 extern "C" int ried_layer_norm_fwd(const void* x, long long ldx, const void* w, const void* b, void* y, long long ldy,
                                    float* mean, float* rstd, long long rows, int C, float eps, int type, int wtype,
@@ -374,7 +376,6 @@ extern "C" int ried_layer_norm_fwd(const void* x, long long ldx, const void* w, 
   if (rows == 0) return RIED_OK;
   RIED_CHECK_ARG(x && y, "ried_layer_norm_fwd: null pointer");
   RIED_CHECK_ARG(ldx >= C && ldy >= C, "ried_layer_norm_fwd: rows overlap (ldx %lld, ldy %lld, %d columns)", ldx, ldy, C);
-  const LnPlan pl = ln_plan(type, C);
   LN_DISPATCH({
 #define LN_FWD(NV, LPR, WPR)                                                                                         \
   hipLaunchKernelGGL((ln_fwd_kernel<T, W, NV, LPR, WPR>), dim3(ceil_div(rows, WPR > 1 ? 1 : 256 / LPR)),             \
@@ -399,7 +400,6 @@ extern "C" int ried_layer_norm_bwd(const void* dy, long long lddy, const void* x
                  "ried_layer_norm_bwd: parameter gradients need ried_layer_norm_bwd_scratch_floats() of scratch");
   const bool sums = dw || db;
   const int nparts = rows > 0 ? ln_parts(rows, type, C) : 0;
-  const LnPlan pl = ln_plan(type, C);
   if (rows > 0) {
     LN_DISPATCH({
 #define LN_BWD(NV, LPR, WPR)                                                                                         \

@@ -153,7 +153,7 @@ extern "C" int ried_rotary(const void* x, long long xb, long long xl, long long 
   A.inv_per = 1.f / (float)(H * A.chunks);
   A.inv_chunks = 1.f / (float)A.chunks;
   const long long blocks = (long long)B * A.lblocks;
-  RIED_CHECK_ARG(blocks <= 0x7fffffffll, "ried_rotary: too many tokens");
+  RIED_CHECK_ARG(blocks < (1ll << 24), "ried_rotary: too many tokens");
   TOK_DISPATCH(type, T, {
 #define ROT_LAUNCH(INTER, WHOLE) hipLaunchKernelGGL((rotary_kernel<T, INTER, WHOLE>), dim3((unsigned)blocks), dim3(256), 0, stream, A)
     if (pairs % V == 0) { if (interleaved) ROT_LAUNCH(true, true); else ROT_LAUNCH(false, true); }

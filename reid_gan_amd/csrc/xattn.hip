@@ -5,9 +5,15 @@
 // and values serves them all.
 #include "xattn.h"
 
+// fp16 weights are held times 2^7 (with the 2^8 that a running maximum may be behind: up to 2^15), so that 2^-31 of the
+// largest still counts beside it; bf16 has fp32's range
+template <typename T> constexpr float xa_up = 0.f;
+template <> constexpr float xa_up<_Float16> = 7.f;
+
 // ---------------------------------------------------------------------------------------------------------------------
-// Tiles: a wave owns 32 rows, a block of NW waves 32 NW; tiles of 64 keys go HBM -> LDS by DMA, one barrier per tile.  S^T = K Q^T leaves a row's scores in one lane pair, so the softmax runs in registers, and P^T is the B operand
-// of O^T += V^T P^T as it stands.  The running maximum is raised only when a score exceeds it by more than 2^8 (the
+// Tiles: a wave owns 32 rows, a block of NW waves 32 NW; tiles of 64 keys go HBM -> LDS by DMA, one barrier per tile.
+// S^T = K Q^T leaves a row's scores in one lane pair, so the softmax runs in registers, and P^T is the B operand of
+// O^T += V^T P^T as it stands.  The running maximum is raised only when a score exceeds it by more than 2^8 (the
 // sums hold that in fp32): rescaling is rare after the first tile.
 // ---------------------------------------------------------------------------------------------------------------------
 template <int DP, int NW> struct XaFwd { static constexpr int STAGES = NW == 8 ? 3 : 2, LDS = STAGES * 2 * 64 * XaTile<DP>::RB; };
@@ -81,12 +87,10 @@ __global__ __launch_bounds__(64 * NW, 2) void xattn_fwd_kernel(XaArgs A) {
     {
       const char* kt = smem + buf * 2 * TILE;
       f32x16 s[2] = {xa_zero(), xa_zero()};
-      
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int u = 0; u < 2; ++u) s[u] = xa_mma<T>(xa_frag<DP>(kt, 32 * u, ks, lane), fq[ks], s[u]);
-      
       if (w[0] != ~0ull) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -104,7 +108,7 @@ __global__ __launch_bounds__(64 * NW, 2) void xattn_fwd_kernel(XaArgs A) {
         float lo, hi;
         xa_halves(mx, lo, hi);
         const float mn = fmaxf(m, fmaxf(lo, hi));
-        const float nc = mn == -INFINITY ? 0.f : mn * c;
+        const float nc = mn == -INFINITY ? 0.f : mn * c - xa_up<T>;
         const float a = xa_exp2((m == -INFINITY ? -INFINITY : mc) - nc);
         m = mn;
         mc = nc;
@@ -119,7 +123,6 @@ __global__ __launch_bounds__(64 * NW, 2) void xattn_fwd_kernel(XaArgs A) {
           s[u][r] = xa_exp2(__builtin_fmaf(s[u][r], c, -mc));
           sum += s[u][r];
         }
-      
       auto add = [&](auto kb_) {
         constexpr int kb = decltype(kb_)::value;
         u32x4 fv[DT];
@@ -129,7 +132,6 @@ __global__ __launch_bounds__(64 * NW, 2) void xattn_fwd_kernel(XaArgs A) {
         for (int d = 0; d < DT; ++d) acc[d] = xa_mma<T>(fv[d], p, acc[d]);
       };
       add(XaInt<0>{}), add(XaInt<1>{}), add(XaInt<2>{}), add(XaInt<3>{});
-      
     }
 #pragma unroll
     for (int i = 0; i < NST - 1; ++i) w[i] = w[i + 1];
@@ -140,7 +142,7 @@ __global__ __launch_bounds__(64 * NW, 2) void xattn_fwd_kernel(XaArgs A) {
   float lo, hi;
   xa_halves(sum, lo, hi);
   const float total = lo + hi;
-  // (zero only for a row without keys: a row's largest weight is at least 1.  NaN goes on to the result.)
+  // (zero only for a row without keys: a row's largest weight is at least 1, or 2^7.  NaN goes on to the result.)
   const float inv = total == 0.f ? 0.f : 1.f / total;
   const float lse = total == 0.f ? -INFINITY : (mc + __log2f(total)) * XA_LN2;
   if (!live) return;
@@ -253,7 +255,7 @@ __global__ __launch_bounds__(256, 1) void xattn_token_kernel(XaArgs A) {
         float lo, hi;
         xa_halves(mx, lo, hi);
         const float mn = fmaxf(m, fmaxf(lo, hi));
-        const float nc = mn == -INFINITY ? 0.f : mn * c;
+        const float nc = mn == -INFINITY ? 0.f : mn * c - xa_up<T>;
         const float a = xa_exp2((m == -INFINITY ? -INFINITY : mc) - nc);
         m = mn;
         mc = nc;
@@ -504,7 +506,7 @@ extern "C" int ried_xattn_fwd(const ried_xattn_t* desc, hipStream_t stream) {
   A.tiles = s.tiles;
   A.nsplit = s.nsplit;
   A.nw = s.nw;
-  RIED_CHECK_ARG((long long)A.tiles * A.nsplit * A.B * A.Hkv <= 0x7fffffffll, "ried_xattn_fwd: too many blocks");
+  RIED_CHECK_ARG((long long)A.tiles * A.nsplit * A.B * A.Hkv * 64 * A.nw < (1ll << 32), "ried_xattn_fwd: too many blocks");
   if (A.nsplit > 1) {
     RIED_CHECK_ARG(d.scratch, "ried_xattn_fwd: this call needs ried_xattn_fwd_scratch_floats() of scratch");
     A.part = d.scratch;

@@ -9,9 +9,6 @@
 // sum_c dO o = sum_j P dP: the stored o is rounded and was formed from rounded weights, which with two keys is off by as
 // much as dP - Dl is large (and with one key dS = 0 is all there is); it is formed from the scores instead, in a first pass
 // over the keys.  And what rounding P and dS to the type leaves over enters the products as a second operand.
-#ifndef XA_WANT_K
-#define XA_WANT_K (d.dim <= 64 ? 1024 : 256)
-#endif
 #define XA_FEW 4
 template <typename T> __device__ __forceinline__ u32x4 xa_rest(const f32x16& s, int which, u32x4 rounded) {
   float f[8];
@@ -67,7 +64,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
   const T* op = (const T*)A.o + (long long)b * A.os[0] + (long long)qi * A.os[1] + (long long)hq * A.os[2];
   const int nk = xa_keys(A, b), ntile = (nk + 63) >> 6, per = (ntile + A.nsplit - 1) / A.nsplit;
   const int t0 = split * per, t1 = t0 + per < ntile ? t0 + per : ntile;
-  const bool few = A.nsplit == 1 && ntile <= XA_FEW;
+  const bool few = ntile <= XA_FEW;
   u32x4 fq[KS], fg[KS];
   float delta = 0.f;
 #pragma unroll
@@ -490,7 +487,7 @@ static XaBwdPlan xa_bwd_plan(const ried_xattn_t& d) {
   p.qtiles = ceil_div(rows, 128);
   p.qsplit = split(p.qtiles * heads, 512, d.keys / 256);
   p.ktiles = ceil_div(d.keys, 64);
-  p.ksplit = split(p.ktiles * heads, XA_WANT_K, rows / 256);
+  p.ksplit = split(p.ktiles * heads, d.dim <= 64 ? 1024 : 256, rows / 256);
   const long long a = p.qsplit > 1 ? p.qsplit * p.rows_all * d.dim : 0, b = p.ksplit > 1 ? 2 * p.ksplit * p.keys_all * d.dim : 0;
   p.floats = 2 * ((p.rows_all + 3) / 4 * 4) + (a > b ? a : b);
   return p;
@@ -548,7 +545,7 @@ extern "C" int ried_xattn_bwd(const ried_xattn_t* desc, hipStream_t stream) {
                    "ried_xattn_bwd: the heads of a group span over 2^31 bytes of q or dout: pass fewer queries");
   XaArgs A = xa_args(d);
   const XaBwdPlan p = xa_bwd_plan(d);
-  RIED_CHECK_ARG((long long)p.qtiles * p.qsplit * A.B * A.Hkv <= 0x7fffffffll && (long long)p.ktiles * p.ksplit * A.B * A.Hkv <= 0x7fffffffll,
+  RIED_CHECK_ARG((long long)p.qtiles * p.qsplit * A.B * A.Hkv < (1ll << 24) && (long long)p.ktiles * p.ksplit * A.B * A.Hkv < (1ll << 23),
                  "ried_xattn_bwd: too many blocks");
   const long long pad = (p.rows_all + 3) / 4 * 4;
   A.lse2 = d.scratch;

@@ -72,6 +72,10 @@ class _Bank:
             _check_param(p)
             if p.numel() != n or p.dtype is not self.dtype or p.device != self.device:
                 raise RuntimeError("AdamW: a parameter changed its size, type or device after the optimizer's first step")
+        width = self.params[0].element_size()
+        spans = sorted((p, p + n * width) for p, n in zip(at, self.sizes) if n)
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("AdamW: two parameters share memory")
         one = 4 if self.bits == 32 else 1                     # bytes of a moment
         m, v = (self.flat[k].data_ptr() for k in self.flat if not k.endswith("_scale"))
         ms, vs = (self.flat[k].data_ptr() for k in self.flat if k.endswith("_scale")) if self.bits == 8 else (0, 0)
@@ -79,7 +83,6 @@ class _Bank:
                 for p, s, n in zip(at, self.starts, self.sizes)]
         self.tables.append(torch.tensor(rows, dtype=torch.int64).to(self.device))
         self.at = at
-
 
     def gradients(self):
         """Addresses of the gradients in self.grads (0: none); returns the copies that stand in for those that are not
@@ -99,10 +102,11 @@ class _Bank:
                 raise TypeError(f"AdamW: gradients are dense and of their parameter's type, not {g.layout} {g.dtype}")
             if g.numel() != n or g.device != self.device:
                 raise ValueError(f"AdamW: a gradient of {g.numel()} elements on {g.device} for a parameter of {n} on {self.device}")
-            if not g.is_contiguous():
-                g = g.contiguous()
+            if not g.is_contiguous() or g.is_neg():
+                g = g.contiguous().resolve_neg()
                 kept.append(g)
             self.grads[i] = g.data_ptr()
+        torch.autograd.graph.increment_version([p for p in self.params if p.grad is not None])
         return kept
 
 
@@ -111,7 +115,7 @@ def _check_param(p: torch.Tensor):
         raise RuntimeError("AdamW: parameters must be on a ROCm device (call .cuda()); there is no CPU path")
     if p.dtype not in (F32, torch.bfloat16):
         raise TypeError(f"AdamW: parameters are fp32 or bf16, not {p.dtype}")
-    if not p.is_contiguous():
+    if not p.is_contiguous() or p.is_neg():
         raise ValueError("AdamW: parameters must be contiguous")
 
 

@@ -354,6 +354,35 @@ def test_cross_attention_many_shares_of_the_keys(keys):
     cross_check(q, k, v, None, mask, train=False)
 
 
+@pytest.mark.parametrize("kind", [BF16, F16])
+def test_cross_attention_one_key_has_no_score_gradient(kind):
+    """With one key that counts the weight is 1 whatever the score: dq and dk are zeros but for the fp32 rounding of dP - Dl
+    (2 D e of |dO||v|), and the key's dv is the sum of dO.  Also where the keys are shared out over several blocks."""
+    for Lq, Lk in ((20, 1), (3, 1200), (200, 700)):
+        q, k, v = (t.requires_grad_() for t in qkv(18, 2, Lq, Lk, 4, 2, 64, kind))
+        lengths = torch.ones(2, dtype=torch.int32, device=DEV)
+        d = normal(gen(19), *q.shape, to=kind)
+        dq, dk, dv = torch.autograd.grad(attention.cross_attention(q, k, v, lengths), (q, k, v), d)
+        size = (d.double().abs().sum(-1) * 5 * 5 * 128 * E).max().item() * 5 * 0.125
+        assert dq.abs().max().item() <= size and dk[:, 0].abs().max().item() <= size * Lq * 2
+        want = d.double().transpose(1, 2).unflatten(1, (2, 2)).sum((2, 3))
+        within(dv[:, 0], want, U[kind] * want.abs() + 4 * Lq * E * d.double().abs().transpose(1, 2).unflatten(1, (2, 2)).sum((2, 3)), "dv")
+
+
+def test_cross_attention_small_weights_add_up_in_half_precision():
+    """40000 keys of weight 2^-25 beside one of weight 1: together 2^-10 of the result.  A weight's rounding is at most
+    2^-25 of its scale, 2^7 here: 40000 * 2^-32 in all, beside the roundings of the scores (e of |s| < 32) and the result."""
+    n = 40000
+    for Lq in (2, 70):                                                        # (single tokens, tiles)
+        q, k, v = (torch.zeros(1, m, 1, 64, dtype=F16, device=DEV) for m in (Lq, n, n))
+        q[..., 0], k[:, 0, :, 0], v[:, 1:] = 1, 17.328, 1
+        s = k[0, 0, 0, 0].double()
+        w = (n - 1) * torch.exp(-s)
+        want = (w / (1 + w)).expand(1, Lq, 1, 64)
+        got = attention.cross_attention(q, k, v, scale=1.0)
+        within(got, want, n * 2 ** -32 + want * (U[F16] + 64 * E + n * E), "small weights")
+
+
 def test_cross_attention_no_keys_no_queries_no_batch():
     for B, Lq, Lk in ((2, 3, 0), (2, 0, 3), (0, 3, 3)):
         q, k, v = (t.requires_grad_() for t in qkv(1, B, Lq, Lk, 4, 2, 64, BF16))
@@ -594,6 +623,59 @@ def test_gradients_under_capture_are_refused():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(kept[0], attention.cross_attention(q, k, v))
+
+
+def test_what_is_written_in_place_counts_as_written():
+    """A graph that saved a tensor refuses to use it once rotary(out=...) or an optimizer step has written it."""
+    g = gen(92)
+    sections = (8, 12, 12)
+    x, pos, freqs = normal(g, 1, 3, 2, 64), torch.ones(1, 3, 3, device=DEV, dtype=torch.int32), attention.rotary_frequencies(sections)
+    w = torch.nn.Parameter(normal(g, 64))
+    y = (x * w).sum()
+    with torch.no_grad():
+        attention.rotary(x, pos, freqs, sections, out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+    for contiguous in (True, False):
+        p = torch.nn.Parameter(normal(g, 8, 8))
+        loss = p.square().sum()
+        p.grad = torch.ones(8, 8, device=DEV) if contiguous else torch.ones(8, 8, device=DEV).t()
+        optim.AdamW([p]).step()
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            loss.backward()
+
+
+def test_adamw_refuses_parameters_that_share_memory():
+    buf = torch.zeros(100, device=DEV)
+    a, b = torch.nn.Parameter(buf[:60]), torch.nn.Parameter(buf[40:])
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    with pytest.raises(ValueError, match="share memory"):
+        optim.AdamW([a, b]).step()
+    c, d = torch.nn.Parameter(buf[:40]), torch.nn.Parameter(buf[40:])         # (side by side is fine)
+    c.grad, d.grad = torch.ones_like(c), torch.ones_like(d)
+    optim.AdamW([c, d], lr=1.0, weight_decay=0.0).step()
+    assert (buf < -0.9).all()
+
+
+def test_lazily_negated_views_are_not_taken_for_their_storage():
+    c = torch.randn(4, 64, dtype=torch.complex64, generator=gen(93), device=DEV).conj().imag
+    assert c.is_neg()
+    with pytest.raises(ValueError, match="resolve_neg"):
+        attention.layer_norm(c)
+    p = torch.nn.Parameter(torch.zeros(4, 64, device=DEV))
+    q = torch.nn.Parameter(torch.zeros(4, 64, device=DEV))
+    p.grad, q.grad = c, c.resolve_neg().contiguous()
+    optim.AdamW([p], lr=1.0).step(), optim.AdamW([q], lr=1.0).step()
+    assert torch.equal(p, q)
+
+
+def test_layer_norm_rows_far_from_zero_with_odd_channels():
+    """Where no channel is, mean * rstd would be infinite: it must not reach the sums of the backward pass."""
+    for C in (13, 1001, 5003):
+        x = torch.full((3, C), 2e38 / C * 0.5, device=DEV).requires_grad_()
+        d = normal(gen(94), 3, C)
+        dx, = torch.autograd.grad(attention.layer_norm(x), x, d)
+        assert torch.isfinite(dx).all(), C
 
 
 # --------------------------------------------------------------------------- AdamW

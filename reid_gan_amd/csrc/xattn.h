@@ -175,7 +175,7 @@ struct XaArgs {
   const int* lengths;
   const unsigned char* mask;
   long long qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3], ms;
-  int B, Lq, Lk, Hkv, G, D, rows, nsplit, tiles, nw;
+  int B, Lq, Lk, Hkv, G, D, rows, nsplit, tiles, nw, ragged;
   float scale;
 };
 

@@ -243,241 +243,383 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// dk, dv: a block owns 64 keys and walks tiles of rows (Q, dO and the rows' two numbers through LDS DMA, two stages); a
-// wave takes 32 of the keys (K and V fragments in registers) and 64 rows of every tile, and the row groups are added
-// through LDS at the end.  Up to 64 channels a block has eight waves (four row groups, two waves per SIMD where the keys
-// give only one block per CU), above that the registers allow four.  S = Q K^T and dP = dO V^T have the row along the registers, so P
-// and dS are the B operands of dv^T += dO^T P and dk^T += Q^T dS as they stand.
+// dk, dv: a block takes 64 keys at a time and walks tiles of rows (Q, dO and the rows' two numbers through LDS DMA, two
+// stages of 128); a wave takes 32 of the keys (K and V fragments in registers) and 64 rows of every tile, and the two row
+// groups are added through LDS at the end.  Registers and LDS allow a CU two blocks up to 64 channels, one above.  (Two
+// blocks of four waves, each with barriers of its own, against one of eight: 60 against 69 us for 4 x 4096 rows over 657
+// to 1500 keys of 4 heads of 64 channels.)  S = Q K^T and dP = dO V^T have the row along the registers, so P and dS are the
+// B operands of dv^T += dO^T P and dk^T += Q^T dS as they stand.
+//
+// The work is (64 keys) x (row tiles) of every batch entry and key head, counted through in that order.  Either a block
+// takes one 64 keys with all rows, or the count is dealt out in even shares, one for every block that the chip holds: a share
+// begins and ends in the middle of some 64 keys' rows, and leaves those two as partial sums that the next kernel adds, in
+// the order of the shares.  With ragged lengths only the 64s that hold keys are counted.
 // ---------------------------------------------------------------------------------------------------------------------
 template <int DP>
-struct XaKv { static constexpr int NW = DP <= 64 ? 8 : 4, RG = NW / 2, ROWS = 64 * RG, STAGE = 2 * ROWS * XaTile<DP>::RB + 8 * ROWS; };
+struct XaKv {
+  static constexpr int NW = 4, RG = NW / 2, ROWS = 64 * RG, BLOCKS = DP <= 64 ? 2 : 1, STAGE = 2 * ROWS * XaTile<DP>::RB + 8 * ROWS;
+};
+#define XA_RAGGED 256                                             // batch entries whose lengths are counted
+// before[b]: 64s with keys in the batch entries before b
+__device__ __forceinline__ void xa_count(const XaArgs& A, int* before) {
+  if (!A.ragged) return;
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    int n[4], s = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      n[i] = lane * 4 + i < A.B ? (xa_keys(A, lane * 4 + i) + 63) >> 6 : 0;
+      s += n[i];
+    }
+    int at = s;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(at, o, 64);
+      if (lane >= o) at += x;
+    }
+    if (lane == 63) before[XA_RAGGED] = at;
+    at -= s;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      before[lane * 4 + i] = at;
+      at += n[i];
+    }
+  }
+  __syncthreads();
+}
+// share i of the count is [i * units / n, (i + 1) * units / n); every share has at least two tiles of rows
+struct XaShares {
+  long long units;
+  int per, n;                                                     // row tiles of 64 keys; shares
+  __device__ __forceinline__ XaShares(const XaArgs& A, const int* before) {
+    per = (A.rows + 127) >> 7;
+    units = (long long)(A.ragged ? __builtin_amdgcn_readfirstlane(before[A.B]) : A.B * A.tiles) * A.Hkv * per;
+    const long long most = units / 2;
+    n = A.nsplit < most ? A.nsplit : most > 0 ? (int)most : units > 0 ? 1 : 0;
+  }
+  __device__ __forceinline__ long long begin(int i) const { return i * units / n; }
+  __device__ __forceinline__ int of(long long unit) const { return (int)(((unit + 1) * n - 1) / units); }
+};
+
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * XaKv<DP>::NW, XaKv<DP>::NW / 4) void xattn_dkv_kernel(XaArgs A) {
+__global__ __launch_bounds__(64 * XaKv<DP>::NW, XaKv<DP>::BLOCKS) void xattn_dkv_kernel(XaArgs A) {
   constexpr int KS = XaTile<DP>::KS, DT = XaTile<DP>::DT, RB = XaTile<DP>::RB, NC = XaTile<DP>::NC, RPI = XaTile<DP>::RPI;
-  constexpr int NW = XaKv<DP>::NW, RG = XaKv<DP>::RG, ROWS = XaKv<DP>::ROWS, TILE = ROWS * RB, NI = ROWS / NW / RPI, STAGE = XaKv<DP>::STAGE;
+  constexpr int NW = XaKv<DP>::NW, RG = XaKv<DP>::RG, ROWS = XaKv<DP>::ROWS, TILE = ROWS * RB, STEP = NW * RPI, NI = ROWS / STEP, STAGE = XaKv<DP>::STAGE;
+  static_assert(ROWS == 128, "row tiles as they are counted");
   constexpr int EX = 2 * DT * 4 * 64;                             // vectors of four a wave hands over
   static_assert((RG - 1) * 2 * EX * 16 <= 2 * STAGE, "the exchange reuses the stages");
   extern __shared__ __align__(16) char smem[];                    // [2][Q tile, dO tile, ROWS lse2, ROWS Dl]
+  __shared__ int before[XA_RAGGED + 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  int inner, head;
-  xa_block(A.tiles * A.nsplit, A.B * A.Hkv, inner, head);
-  const int b = head / A.Hkv, hk = head % A.Hkv, tile = inner % A.tiles, split = inner / A.tiles;
-  const int grp = wave >> 1, key = tile * 64 + (wave & 1) * 32 + (lane & 31);
-  const int nk = xa_keys(A, b);
-  const bool counts = key < nk && (!A.mask || A.mask[(long long)b * A.ms + key]);
-  const T* kp = (const T*)A.k + (long long)b * A.ks[0] + (long long)key * A.ks[1] + (long long)hk * A.ks[2];
-  const T* vp = (const T*)A.v + (long long)b * A.vs[0] + (long long)key * A.vs[1] + (long long)hk * A.vs[2];
-  u32x4 fk[KS], fv[KS];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const int d = s * 16 + h * 8;
-    const bool ok = counts && d < A.D;
-    fk[s] = ok ? *reinterpret_cast<const u32x4*>(kp + d) : u32x4{0, 0, 0, 0};
-    fv[s] = ok ? *reinterpret_cast<const u32x4*>(vp + d) : u32x4{0, 0, 0, 0};
+  const int grp = wave >> 1;
+  xa_count(A, before);
+  long long unit, end;
+  int per, share = 0;
+  if (A.nsplit == 0) {                                            // a block, a head's 64 keys
+    int inner, head;
+    xa_block(A.tiles, A.B * A.Hkv, inner, head);
+    per = (A.rows + 127) >> 7;
+    unit = ((long long)head * A.tiles + inner) * per;
+    end = unit + per;
+  } else {
+    const XaShares S(A, before);
+    const int id = blockIdx.x, n = gridDim.x;
+    share = (n & 7) == 0 ? (id & 7) * (n >> 3) + (id >> 3) : id;  // (neighbours on one XCD)
+    if (share >= S.n) return;
+    per = S.per;
+    unit = S.begin(share);
+    end = S.begin(share + 1);
   }
-  const int ntile = (A.rows + ROWS - 1) / ROWS, per = (ntile + A.nsplit - 1) / A.nsplit;
-  const int t0 = split * per;
-  int t1 = t0 + per < ntile ? t0 + per : ntile;
-  if (tile * 64 >= nk) t1 = t0;                                   // no key here counts: zeros
-  const char* qp = (const char*)((const T*)A.q + (long long)b * A.qs[0] + (long long)hk * A.G * A.qs[2]);
-  const char* gp = (const char*)((const T*)A.dout + (long long)b * A.gs[0] + (long long)hk * A.G * A.gs[2]);
-  const __amdgpu_buffer_rsrc_t rq = xa_rsrc(qp), rg = xa_rsrc(gp);   // (host-checked: the heads of a group stay below 2^31 bytes)
-  const __amdgpu_buffer_rsrc_t rl = xa_rsrc(A.lse2 + (long long)head * A.rows), rd = xa_rsrc(A.delta + (long long)head * A.rows);
+  const float c = A.scale * XA_LOG2E;
   const int qrow = (int)A.qs[1] * 2, qhead = (int)A.qs[2] * 2, grow = (int)A.gs[1] * 2, ghead = (int)A.gs[2] * 2;
   const int srow = wave * RPI + lane / NC, sc = (lane % NC) ^ xa_swz<RB>(srow);
   const unsigned dead = sc * 8 >= A.D ? XA_OOB : 0u;
   const float inv_lq = 1.f / (float)A.Lq;
-  auto issue = [&](int t, int buf) {
-    char* st = smem + buf * STAGE;
-    char* dst = st + wave * RPI * RB;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int r = t * ROWS + srow + i * NW * RPI;
-      int qi;
-      const int g = fast_div(r, A.Lq, inv_lq, qi);
-      const unsigned bad = (r < A.rows ? 0u : XA_OOB) | dead;
-      xa_dma16(rq, (unsigned)(qi * qrow + g * qhead + sc * 16) | bad, 0, dst + i * NW * RPI * RB);
-      xa_dma16(rg, (unsigned)(qi * grow + g * ghead + sc * 16) | bad, 0, dst + TILE + i * NW * RPI * RB);
+  const int sg = STEP / A.Lq, sr = STEP - sg * A.Lq;              // STEP rows on: sg heads and sr rows, or a head more
+  const unsigned qstep = (unsigned)(sr * qrow) + (unsigned)sg * (unsigned)qhead, gstep = (unsigned)(sr * grow) + (unsigned)sg * (unsigned)ghead;
+  const unsigned qover = qstep + (unsigned)qhead - (unsigned)A.Lq * (unsigned)qrow, gover = gstep + (unsigned)ghead - (unsigned)A.Lq * (unsigned)grow;
+  while (unit < end) {
+    const long long flat = unit / per;                            // which 64 keys
+    const int t0 = (int)(unit - flat * per);
+    int t1 = end - unit < per - t0 ? t0 + (int)(end - unit) : per;
+    const bool whole = t0 == 0 && t1 == per;
+    unit += t1 - t0;
+    int b, hk, tile;
+    if (A.ragged) {
+      int lo = 0, hi = A.B;                                       // the last entry that begins at `flat` or before it
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if ((long long)__builtin_amdgcn_readfirstlane(before[mid]) * A.Hkv <= flat) lo = mid; else hi = mid;
+      }
+      const int first = __builtin_amdgcn_readfirstlane(before[lo]), many = __builtin_amdgcn_readfirstlane(before[lo + 1]) - first;
+      const int in = (int)(flat - (long long)first * A.Hkv);
+      b = lo;
+      hk = in / many;
+      tile = in - hk * many;
+    } else {
+      const int head = (int)(flat / A.tiles);
+      tile = (int)(flat - (long long)head * A.tiles);
+      b = head / A.Hkv;
+      hk = head - b * A.Hkv;
     }
-    const int part = wave % RG, r = t * ROWS + part * 64 + lane;
-    const unsigned off = r < A.rows ? (unsigned)r * 4u : XA_OOB;
-    if (wave < RG) xa_dma4(rl, off, st + 2 * TILE + part * 256);
-    else xa_dma4(rd, off, st + 2 * TILE + 4 * ROWS + part * 256);
-  };
-  const float c = A.scale * XA_LOG2E;
-  const bool few = nk <= 64 * XA_FEW;
-  float es = XaRange<T>::on ? 0x1p9f : 1.f;                       // (times the 2^15 of P)
-  f32x16 dv[DT], dk[DT];
+    const long long head = (long long)b * A.Hkv + hk;
+    const int key = tile * 64 + (wave & 1) * 32 + (lane & 31), nk = xa_keys(A, b);
+    const bool counts = key < nk && (!A.mask || A.mask[(long long)b * A.ms + key]);
+    const T* kp = (const T*)A.k + (long long)b * A.ks[0] + (long long)key * A.ks[1] + (long long)hk * A.ks[2];
+    const T* vp = (const T*)A.v + (long long)b * A.vs[0] + (long long)key * A.vs[1] + (long long)hk * A.vs[2];
+    u32x4 fk[KS], fv[KS];
 #pragma unroll
-  for (int d = 0; d < DT; ++d) dv[d] = dk[d] = xa_zero();
-  XaTr<DP> tr(smem + grp * 64 * RB, lane);
-  auto rows = [&](auto few_) {
-    int buf = 0;
-    if (t0 < t1) issue(t0, 0);
-    for (int t = t0; t < t1; ++t) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      if (t + 1 < t1) issue(t + 1, buf ^ 1);
-      const char* qt = smem + buf * STAGE + grp * 64 * RB;
-      const char* gt = qt + TILE;
-      const float* rowv = reinterpret_cast<const float*>(smem + buf * STAGE + 2 * TILE) + grp * 64;
-      auto rows32 = [&](auto u_) {
-        constexpr int u = decltype(u_)::value;
-        f32x16 s = xa_zero(), dp = xa_zero();
+    for (int s = 0; s < KS; ++s) {
+      const int d = s * 16 + h * 8;
+      const bool ok = counts && d < A.D;
+      fk[s] = ok ? *reinterpret_cast<const u32x4*>(kp + d) : u32x4{0, 0, 0, 0};
+      fv[s] = ok ? *reinterpret_cast<const u32x4*>(vp + d) : u32x4{0, 0, 0, 0};
+    }
+    if (tile * 64 >= nk) t1 = t0;                                 // no key here counts: zeros
+    const char* qp = (const char*)((const T*)A.q + (long long)b * A.qs[0] + (long long)hk * A.G * A.qs[2]);
+    const char* gp = (const char*)((const T*)A.dout + (long long)b * A.gs[0] + (long long)hk * A.G * A.gs[2]);
+    const __amdgpu_buffer_rsrc_t rq = xa_rsrc(qp), rg = xa_rsrc(gp);   // (host-checked: the heads of a group stay below 2^31 bytes)
+    const __amdgpu_buffer_rsrc_t rl = xa_rsrc(A.lse2 + head * A.rows), rd = xa_rsrc(A.delta + head * A.rows);
+    // where this lane's next row of Q and of dO lies: tiles are asked for in order, STEP rows an instruction
+    int qi;
+    const int g0 = fast_div(t0 * ROWS + srow, A.Lq, inv_lq, qi);
+    unsigned oq = (unsigned)qi * (unsigned)qrow + (unsigned)g0 * (unsigned)qhead + (unsigned)(sc * 16);
+    unsigned og = (unsigned)qi * (unsigned)grow + (unsigned)g0 * (unsigned)ghead + (unsigned)(sc * 16);
+    auto issue = [&](int t, int buf) {
+      char* st = smem + buf * STAGE;
+      char* dst = st + wave * RPI * RB;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          s = xa_mma<T>(xa_frag<DP>(qt, 32 * u, ks, lane), fk[ks], s);
-          dp = xa_mma<T>(xa_frag<DP>(gt, 32 * u, ks, lane), fv[ks], dp);
-        }
-        float mx = 0.f;
+      for (int i = 0; i < NI; ++i) {
+        const unsigned bad = (srow < A.rows - t * ROWS - i * STEP ? 0u : XA_OOB) | dead;
+        xa_dma16(rq, oq | bad, 0, dst + i * STEP * RB);
+        xa_dma16(rg, og | bad, 0, dst + TILE + i * STEP * RB);
+        qi += sr;
+        const bool over = qi >= A.Lq;
+        qi -= over ? A.Lq : 0;
+        oq += over ? qover : qstep;
+        og += over ? gover : gstep;
+      }
+      const int part = wave % RG, r = t * ROWS + part * 64 + lane;
+      const unsigned off = r < A.rows ? (unsigned)r * 4u : XA_OOB;
+      if (wave < RG) xa_dma4(rl, off, st + 2 * TILE + part * 256);
+      else xa_dma4(rd, off, st + 2 * TILE + 4 * ROWS + part * 256);
+    };
+    const bool few = nk <= 64 * XA_FEW;
+    float es = XaRange<T>::on ? 0x1p9f : 1.f;                     // (times the 2^15 of P)
+    f32x16 dv[DT], dk[DT];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 l4 = *reinterpret_cast<const f32x4*>(rowv + 32 * u + 8 * q + 4 * h);
-          const f32x4 d4 = *reinterpret_cast<const f32x4*>(rowv + ROWS + 32 * u + 8 * q + 4 * h);
+    for (int d = 0; d < DT; ++d) dv[d] = dk[d] = xa_zero();
+    XaTr<DP> tr(smem + grp * 64 * RB, lane);
+    auto rows = [&](auto few_) {
+      int buf = 0;
+      if (t0 < t1) issue(t0, 0);
+      for (int t = t0; t < t1; ++t) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (t + 1 < t1) issue(t + 1, buf ^ 1);
+        const char* qt = smem + buf * STAGE + grp * 64 * RB;
+        const char* gt = qt + TILE;
+        const float* rowv = reinterpret_cast<const float*>(smem + buf * STAGE + 2 * TILE) + grp * 64;
+        auto rows32 = [&](auto u_) {
+          constexpr int u = decltype(u_)::value;
+          f32x16 s = xa_zero(), dp = xa_zero();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 4 * q + i;
-            s[r] = xa_exp2(__builtin_fmaf(s[r], c, l4[i]));
-            dp[r] = s[r] * (dp[r] - d4[i]);
-            if constexpr (XaRange<T>::on) mx = fmaxf(mx, fabsf(dp[r]));
+          for (int ks = 0; ks < KS; ++ks) {
+            s = xa_mma<T>(xa_frag<DP>(qt, 32 * u, ks, lane), fk[ks], s);
+            dp = xa_mma<T>(xa_frag<DP>(gt, 32 * u, ks, lane), fv[ks], dp);
           }
-        }
-        if constexpr (XaRange<T>::on) {
-          xa_fit<DT>(counts ? mx : 0.f, es, dk);                    // (a hidden key's column is dropped: any size)
+          float mx = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) dp[r] *= es;
-        }
-        auto add = [&](auto kb_) {
-          constexpr int kb = decltype(kb_)::value;
-          u32x4 fg[DT], fq[DT];
-          xa_tr_frags<DP, u * 32 + kb * 16, TILE>(tr, fg);
-          const u32x4 fp = xa_as_b<T>(s, kb);
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(rowv + 32 * u + 8 * q + 4 * h);
+            const f32x4 d4 = *reinterpret_cast<const f32x4*>(rowv + ROWS + 32 * u + 8 * q + 4 * h);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) dv[d] = xa_mma<T>(fg[d], fp, dv[d]);
-          if constexpr (decltype(few_)::value) {
-            const u32x4 rest = xa_rest<T>(s, kb, fp);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) dv[d] = xa_mma<T>(fg[d], rest, dv[d]);
+            for (int i = 0; i < 4; ++i) {
+              const int r = 4 * q + i;
+              s[r] = xa_exp2(__builtin_fmaf(s[r], c, l4[i]));
+              dp[r] = s[r] * (dp[r] - d4[i]);
+              if constexpr (XaRange<T>::on) mx = fmaxf(mx, fabsf(dp[r]));
+            }
           }
-          xa_tr_frags<DP, u * 32 + kb * 16>(tr, fq);
-          const u32x4 fs = xa_as_b<T>(dp, kb);
+          if constexpr (XaRange<T>::on) {
+            xa_fit<DT>(counts ? mx : 0.f, es, dk);                    // (a hidden key's column is dropped: any size)
 #pragma unroll
-          for (int d = 0; d < DT; ++d) dk[d] = xa_mma<T>(fq[d], fs, dk[d]);
-          if constexpr (decltype(few_)::value) {
-            const u32x4 rest = xa_rest<T>(dp, kb, fs);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) dk[d] = xa_mma<T>(fq[d], rest, dk[d]);
+            for (int r = 0; r < 16; ++r) dp[r] *= es;
           }
+          auto add = [&](auto kb_) {
+            constexpr int kb = decltype(kb_)::value;
+            u32x4 fg[DT], fq[DT];
+            xa_tr_frags<DP, u * 32 + kb * 16, TILE>(tr, fg);
+            const u32x4 fp = xa_as_b<T>(s, kb);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dv[d] = xa_mma<T>(fg[d], fp, dv[d]);
+            if constexpr (decltype(few_)::value) {
+              const u32x4 rest = xa_rest<T>(s, kb, fp);
+#pragma unroll
+              for (int d = 0; d < DT; ++d) dv[d] = xa_mma<T>(fg[d], rest, dv[d]);
+            }
+            xa_tr_frags<DP, u * 32 + kb * 16>(tr, fq);
+            const u32x4 fs = xa_as_b<T>(dp, kb);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dk[d] = xa_mma<T>(fq[d], fs, dk[d]);
+            if constexpr (decltype(few_)::value) {
+              const u32x4 rest = xa_rest<T>(dp, kb, fs);
+#pragma unroll
+              for (int d = 0; d < DT; ++d) dk[d] = xa_mma<T>(fq[d], rest, dk[d]);
+            }
+          };
+          add(XaInt<0>{}), add(XaInt<1>{});
         };
-        add(XaInt<0>{}), add(XaInt<1>{});
-      };
-      rows32(XaInt<0>{}), rows32(XaInt<1>{});
-      tr.move(buf ? -STAGE : STAGE);
-      buf ^= 1;
-    }
-  };
-  if (few) rows(XaInt<1>{});
-  else rows(XaInt<0>{});
-  // the other row groups' sums go to the first group's waves, added in order
-  const float fk_ = A.scale * XaRange<T>::p_down / es, fv_ = XaRange<T>::p_down;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  f32x4* ex = reinterpret_cast<f32x4*>(smem) + (wave & 1) * EX + lane;
-#pragma unroll
-  for (int d = 0; d < DT; ++d) {
-    dk[d] *= fk_;
-    dv[d] *= fv_;
-    if (grp) {
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        f32x4* to = ex + (grp - 1) * 2 * EX + (d * 4 + (r >> 2)) * 64;
-        to[0] = f32x4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
-        to[DT * 4 * 64] = f32x4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+        rows32(XaInt<0>{}), rows32(XaInt<1>{});
+        tr.move(buf ? -STAGE : STAGE);
+        buf ^= 1;
       }
-    }
-  }
-  __syncthreads();
-  if (grp || key >= A.Lk) return;
+    };
+    if (few) rows(XaInt<1>{});
+    else rows(XaInt<0>{});
+    // the other row groups' sums go to the first group's waves, added in order
+    const float fk_ = A.scale * XaRange<T>::p_down / es, fv_ = XaRange<T>::p_down;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    f32x4* ex = reinterpret_cast<f32x4*>(smem) + (wave & 1) * EX + lane;
 #pragma unroll
-  for (int o = 0; o < RG - 1; ++o)
+    for (int d = 0; d < DT; ++d) {
+      dk[d] *= fk_;
+      dv[d] *= fv_;
+      if (grp) {
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const f32x4* from = ex + o * 2 * EX + (d * 4 + (r >> 2)) * 64;
-        const f32x4 a = from[0], b = from[DT * 4 * 64];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { dk[d][r + i] += a[i]; dv[d][r + i] += b[i]; }
-      }
-  // (a hidden key's column was computed from zeros and is dropped, whatever it holds)
-  if (!counts) {
-#pragma unroll
-    for (int d = 0; d < DT; ++d) dk[d] = dv[d] = xa_zero();
-  }
-  if (A.nsplit == 1) {
-    T* pk = (T*)A.dk + (long long)b * A.dks[0] + (long long)key * A.dks[1] + (long long)hk * A.dks[2];
-    T* pv = (T*)A.dv + (long long)b * A.dvs[0] + (long long)key * A.dvs[1] + (long long)hk * A.dvs[2];
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int ch = d * 32 + 2 * r + 4 * h;
-        if (ch < A.D) {
-          *reinterpret_cast<u32x2*>(pk + ch) = u32x2{xa_pack<T>(dk[d][r], dk[d][r + 1]), xa_pack<T>(dk[d][r + 2], dk[d][r + 3])};
-          *reinterpret_cast<u32x2*>(pv + ch) = u32x2{xa_pack<T>(dv[d][r], dv[d][r + 1]), xa_pack<T>(dv[d][r + 2], dv[d][r + 3])};
+        for (int r = 0; r < 16; r += 4) {
+          f32x4* to = ex + (grp - 1) * 2 * EX + (d * 4 + (r >> 2)) * 64;
+          to[0] = f32x4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
+          to[DT * 4 * 64] = f32x4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
         }
       }
-  } else {
-    const long long all = (long long)A.B * A.Hkv * A.Lk, at = (long long)split * all + (long long)head * A.Lk + key;
-    float* pk = A.part + at * A.D;
-    float* pv = pk + A.nsplit * all * A.D;
+    }
+    __syncthreads();
+    if (!grp && key < A.Lk) {
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+      for (int o = 0; o < RG - 1; ++o)
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int ch = d * 32 + 2 * r + 4 * h;
-        if (ch < A.D) {
-          *reinterpret_cast<f32x4*>(pk + ch) = f32x4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
-          *reinterpret_cast<f32x4*>(pv + ch) = f32x4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
-        }
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; r += 4) {
+            const f32x4* from = ex + o * 2 * EX + (d * 4 + (r >> 2)) * 64;
+            const f32x4 x = from[0], y = from[DT * 4 * 64];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { dk[d][r + i] += x[i]; dv[d][r + i] += y[i]; }
+          }
+      // (a hidden key's column was computed from zeros and is dropped, whatever it holds)
+      if (!counts) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) dk[d] = dv[d] = xa_zero();
       }
+      if (whole) {
+        T* pk = (T*)A.dk + (long long)b * A.dks[0] + (long long)key * A.dks[1] + (long long)hk * A.dks[2];
+        T* pv = (T*)A.dv + (long long)b * A.dvs[0] + (long long)key * A.dvs[1] + (long long)hk * A.dvs[2];
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; r += 4) {
+            const int ch = d * 32 + 2 * r + 4 * h;
+            if (ch < A.D) {
+              *reinterpret_cast<u32x2*>(pk + ch) = u32x2{xa_pack<T>(dk[d][r], dk[d][r + 1]), xa_pack<T>(dk[d][r + 2], dk[d][r + 3])};
+              *reinterpret_cast<u32x2*>(pv + ch) = u32x2{xa_pack<T>(dv[d][r], dv[d][r + 1]), xa_pack<T>(dv[d][r + 2], dv[d][r + 3])};
+            }
+          }
+      } else {                                                    // [share][rows' begin left out, or their end][dk, dv][64][D]
+        float* pk = A.part + ((2ll * share + (t0 == 0)) * 128 + (key & 63)) * A.D;
+        float* pv = pk + 64 * A.D;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; r += 4) {
+            const int ch = d * 32 + 2 * r + 4 * h;
+            if (ch < A.D) {
+              *reinterpret_cast<f32x4*>(pk + ch) = f32x4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
+              *reinterpret_cast<f32x4*>(pv + ch) = f32x4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+            }
+          }
+      }
+    }
+    __syncthreads();                                              // (the exchange has been read: the stages are free)
   }
 }
 
-// adds the shares up (dq, or dk and dv by blockIdx.y): out[b][l][head in group][d] over rows = G * L of each of the B * Hkv heads, 8 channels per thread
-struct XaSum { void* out; long long sb, sl, sh; };
+// adds the parts of 64 keys whose rows were dealt to several shares; dk or dv by blockIdx.y.  Where lengths are counted, also
+// the zeros of the 64s without keys.
 template <typename T>
-__global__ __launch_bounds__(256) void xattn_sum_kernel(const float* __restrict__ part, int nsplit, int heads, int Hkv, int G,
-                                                        int L, int D, XaSum first, XaSum second) {
-  const XaSum S = blockIdx.y ? second : first;
-  part += (long long)blockIdx.y * nsplit * heads * G * L * D;
-  const int chunks = D >> 3, rows = G * L;
-  const long long all = (long long)heads * rows, i = blockIdx.x * 256ll + threadIdx.x;
+__global__ __launch_bounds__(256) void xattn_parts_kernel(XaArgs A) {
+  __shared__ int before[XA_RAGGED + 1];
+  xa_count(A, before);
+  const XaShares S(A, before);
+  const int head = blockIdx.x / A.tiles, tile = blockIdx.x - head * A.tiles, b = head / A.Hkv, hk = head - b * A.Hkv;
+  long long flat = blockIdx.x;
+  bool none = false;
+  if (A.ragged) {
+    const int many = before[b + 1] - before[b];
+    flat = (long long)before[b] * A.Hkv + (long long)hk * many + tile;
+    none = tile >= many;
+  }
+  int s0 = 0, s1 = 0;
+  if (!none) {
+    s0 = S.of(flat * S.per);
+    s1 = S.of(flat * S.per + S.per - 1);
+    if (s0 == s1) return;                                         // (written whole)
+  }
+  const int chunks = A.D >> 3, which = blockIdx.y;
+  T* out = (T*)(which ? A.dv : A.dk);
+  const long long* st = which ? A.dvs : A.dks;
+  for (int i = threadIdx.x; i < 64 * chunks; i += 256) {
+    const int k = i / chunks, d = (i - k * chunks) * 8, key = tile * 64 + k;
+    if (key >= A.Lk) break;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+    if (!none) {
+      const float* p = A.part + ((2ll * s0 + 1) * 128 + which * 64 + k) * A.D + d;
+      x = *reinterpret_cast<const f32x4*>(p);
+      y = *reinterpret_cast<const f32x4*>(p + 4);
+      for (int s = s0 + 1; s <= s1; ++s) {
+        p = A.part + (2ll * s * 128 + which * 64 + k) * A.D + d;
+        x += *reinterpret_cast<const f32x4*>(p);
+        y += *reinterpret_cast<const f32x4*>(p + 4);
+      }
+    }
+    *reinterpret_cast<u32x4*>(out + (long long)b * st[0] + (long long)key * st[1] + (long long)hk * st[2] + d) =
+        u32x4{xa_pack<T>(x[0], x[1]), xa_pack<T>(x[2], x[3]), xa_pack<T>(y[0], y[1]), xa_pack<T>(y[2], y[3])};
+  }
+}
+
+// adds the shares of dq up, 8 channels per thread
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_sum_kernel(XaArgs A) {
+  const int chunks = A.D >> 3;
+  const long long all = (long long)A.B * A.Hkv * A.rows, i = blockIdx.x * 256ll + threadIdx.x;
   if (i >= all * chunks) return;
   const long long flat = i / chunks;
   const int d = (int)(i - flat * chunks) * 8;
   f32x4 a = {0.f, 0.f, 0.f, 0.f}, e = a;
-  for (int s = 0; s < nsplit; ++s) {
-    const float* p = part + (s * all + flat) * D + d;
+  for (int s = 0; s < A.nsplit; ++s) {
+    const float* p = A.part + (s * all + flat) * A.D + d;
     a += *reinterpret_cast<const f32x4*>(p);
     e += *reinterpret_cast<const f32x4*>(p + 4);
   }
-  const int head = (int)(flat / rows), row = (int)(flat - (long long)head * rows);
-  const int b = head / Hkv, hk = head % Hkv, g = row / L, l = row - g * L;
-  *reinterpret_cast<u32x4*>((T*)S.out + b * S.sb + l * S.sl + (long long)(hk * G + g) * S.sh + d) =
+  const int head = (int)(flat / A.rows), row = (int)(flat - (long long)head * A.rows);
+  const int b = head / A.Hkv, hk = head % A.Hkv, g = row / A.Lq, l = row - g * A.Lq;
+  *reinterpret_cast<u32x4*>((T*)A.dq + b * A.dqs[0] + l * A.dqs[1] + (long long)(hk * A.G + g) * A.dqs[2] + d) =
       u32x4{xa_pack<T>(a[0], a[1]), xa_pack<T>(a[2], a[3]), xa_pack<T>(e[0], e[1]), xa_pack<T>(e[2], e[3])};
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------------
-struct XaBwdPlan { int qtiles, qsplit, ktiles, ksplit; long long rows_all, keys_all, floats; };
+// dk, dv: shares (0: a block for each 64 keys).  Counted in row tiles a block walks one after the other, with `slots` blocks at
+// a time: whole 64s cost ceil(64s / slots) times their rows; shares an even part, and adding their ends up is worth about
+// three tiles more (7.8 us, at 2.8 us a tile).  With lengths, three quarters of the keys are expected to count.
+struct XaBwdPlan { int qtiles, qsplit, ktiles, shares; long long rows_all; };
 static XaBwdPlan xa_bwd_plan(const ried_xattn_t& d) {
   const long long rows = d.heads / d.groups * d.queries, heads = d.batch * d.groups;
   XaBwdPlan p;
   p.rows_all = heads * rows;
-  p.keys_all = heads * d.keys;
   auto split = [](long long blocks, long long want, long long most) {
     long long n = want / (blocks > 0 ? blocks : 1);
     if (n > most) n = most;
@@ -487,9 +629,10 @@ static XaBwdPlan xa_bwd_plan(const ried_xattn_t& d) {
   p.qtiles = ceil_div(rows, 128);
   p.qsplit = split(p.qtiles * heads, 512, d.keys / 256);
   p.ktiles = ceil_div(d.keys, 64);
-  p.ksplit = split(p.ktiles * heads, d.dim <= 64 ? 1024 : 256, rows / 256);
-  const long long a = p.qsplit > 1 ? p.qsplit * p.rows_all * d.dim : 0, b = p.ksplit > 1 ? 2 * p.ksplit * p.keys_all * d.dim : 0;
-  p.floats = 2 * ((p.rows_all + 3) / 4 * 4) + (a > b ? a : b);
+  const long long slots = d.dim <= 64 ? 512 : 256, per = ceil_div(rows, 128), all = p.ktiles * heads, units = all * per;
+  const long long dealt = (d.lengths ? units - units / 4 : units) / slots + 3, kept = ((d.lengths ? all - all / 4 : all) + slots - 1) / slots * per;
+  const long long most = units / 2;
+  p.shares = dealt < kept && most > 1 && (!d.lengths || d.batch <= XA_RAGGED) ? (int)(most < slots ? most : slots) : 0;
   return p;
 }
 
@@ -498,7 +641,12 @@ extern "C" long long ried_xattn_bwd_scratch_floats(long long batch, long long qu
   if (batch <= 0 || queries <= 0 || heads <= 0 || groups <= 0 || heads % groups) return 0;
   ried_xattn_t d = {};
   d.batch = batch; d.queries = queries; d.keys = keys; d.heads = heads; d.groups = groups; d.dim = dim;
-  return xa_bwd_plan(d).floats;
+  const XaBwdPlan p = xa_bwd_plan(d);
+  const int some = 0;
+  d.lengths = &some;                                              // (a plan with lengths may deal where one without does not)
+  const int shares = p.shares ? p.shares : xa_bwd_plan(d).shares;
+  const long long a = p.qsplit > 1 ? p.qsplit * p.rows_all * dim : 0, b = 256ll * shares * dim;
+  return 2 * ((p.rows_all + 3) / 4 * 4) + (a > b ? a : b);
 }
 
 template <typename T, int DP>
@@ -514,16 +662,14 @@ static int xa_bwd_launch(XaArgs A, const XaBwdPlan& p, hipStream_t stream) {
   A.nsplit = p.qsplit;
   hipLaunchKernelGGL((xattn_dq_kernel<T, DP>), dim3((unsigned)(A.tiles * A.nsplit * heads)), dim3(256), lq, stream, A);
   if (A.nsplit > 1)
-    hipLaunchKernelGGL((xattn_sum_kernel<T>), dim3(ceil_div(p.rows_all * (A.D >> 3), 256)), dim3(256), 0, stream, A.part,
-                       A.nsplit, heads, A.Hkv, A.G, A.Lq, A.D, XaSum{A.dq, A.dqs[0], A.dqs[1], A.dqs[2]}, XaSum{});
+    hipLaunchKernelGGL((xattn_sum_kernel<T>), dim3(ceil_div(p.rows_all * (A.D >> 3), 256)), dim3(256), 0, stream, A);
   if (A.Lk == 0) return RIED_OK;
   A.tiles = p.ktiles;
-  A.nsplit = p.ksplit;
-  hipLaunchKernelGGL((xattn_dkv_kernel<T, DP>), dim3((unsigned)(A.tiles * A.nsplit * heads)), dim3(64 * XaKv<DP>::NW), lk, stream, A);
-  if (A.nsplit > 1)
-    hipLaunchKernelGGL((xattn_sum_kernel<T>), dim3(ceil_div(p.keys_all * (A.D >> 3), 256), 2), dim3(256), 0, stream, A.part,
-                       A.nsplit, heads, A.Hkv, 1, A.Lk, A.D, XaSum{A.dk, A.dks[0], A.dks[1], A.dks[2]},
-                       XaSum{A.dv, A.dvs[0], A.dvs[1], A.dvs[2]});
+  A.nsplit = p.shares;
+  A.ragged = p.shares && A.lengths;
+  hipLaunchKernelGGL((xattn_dkv_kernel<T, DP>), dim3((unsigned)(p.shares ? p.shares : A.tiles * heads)), dim3(64 * XaKv<DP>::NW), lk, stream, A);
+  if (p.shares)
+    hipLaunchKernelGGL((xattn_parts_kernel<T>), dim3((unsigned)(A.tiles * heads), 2), dim3(256), 0, stream, A);
   return RIED_OK;
 }
 template <typename T>
@@ -545,7 +691,7 @@ extern "C" int ried_xattn_bwd(const ried_xattn_t* desc, hipStream_t stream) {
                    "ried_xattn_bwd: the heads of a group span over 2^31 bytes of q or dout: pass fewer queries");
   XaArgs A = xa_args(d);
   const XaBwdPlan p = xa_bwd_plan(d);
-  RIED_CHECK_ARG((long long)p.qtiles * p.qsplit * A.B * A.Hkv < (1ll << 24) && (long long)p.ktiles * p.ksplit * A.B * A.Hkv < (1ll << 23),
+  RIED_CHECK_ARG((long long)p.qtiles * p.qsplit * A.B * A.Hkv < (1ll << 24) && (long long)p.ktiles * A.B * A.Hkv < (1ll << 23),
                  "ried_xattn_bwd: too many blocks");
   const long long pad = (p.rows_all + 3) / 4 * 4;
   A.lse2 = d.scratch;

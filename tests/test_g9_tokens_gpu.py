@@ -354,6 +354,23 @@ def test_cross_attention_many_shares_of_the_keys(keys):
     cross_check(q, k, v, None, mask, train=False)
 
 
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("sizes", [(3, 700, 300, 4, 2), (5, 260, 1500, 2, 1), (1, 3000, 70, 4, 4), (2, 1100, 130, 12, 3),
+                                   (300, 40, 65, 2, 2)])
+def test_cross_attention_gradients_of_the_keys_in_shares(sizes, dim):
+    """The keys' gradients where their rows are dealt out to blocks: few and many keys, entries without any between others,
+    whole 64s without keys behind the last one, more entries than are counted."""
+    B, Lq, Lk, H, G = sizes
+    q, k, v = qkv(dim + B, B, Lq, Lk, H, G, dim, BF16)
+    cross_check(q, k, v)
+    lengths = torch.randint(0, Lk + 1, (B,), generator=gen(97), device=DEV, dtype=torch.int32)
+    lengths[B // 2] = 0
+    lengths[B - 1] = Lk if B > 1 else Lk // 2
+    cross_check(q, k, v, lengths)
+    lengths.zero_()
+    cross_check(q, k, v, lengths)
+
+
 @pytest.mark.parametrize("kind", [BF16, F16])
 def test_cross_attention_one_key_has_no_score_gradient(kind):
     """With one key that counts the weight is 1 whatever the score: dq and dk are zeros but for the fp32 rounding of dP - Dl

@@ -10,6 +10,9 @@
 // takes whole blocks of 256 (four elements per lane, four blocks in flight), so a block's maximum is one wave reduction
 // in registers.  Every operation on the moments is rounded by itself (no contraction): the codes do not depend on how the
 // compiler fuses, and an elementwise evaluation in 32 bits gives the same bits.
+// Measured: 222 fp32 tensors of 16 to 524288 elements, 315 MB: 65 us (4.8 TB/s) + 2.6 for the step counts; 48 bf16 tensors of
+// up to 16777216 elements with 8-bit moments, 747 MB: 149 to 154 us (4.9 TB/s; a copy of 1 GB runs at 5.1).  All of a
+// workgroup's loads are in flight before the first is used: with a branch between them 75 and 179 us.
 #include "tokens.h"
 
 #define ADAMW_TENSORS 440    // gradient pointers per launch: they travel as kernel arguments (3.5 of the 4 KB)

@@ -6,6 +6,12 @@
 // squares, so a large mean costs no precision.  The weight's gradient is summed where the row already is: every lane
 // keeps the sums of its own columns over all rows its block takes, the block adds its row groups in LDS, and a second
 // kernel adds the blocks' partial rows.  No atomics: the order of every sum is fixed.
+//
+// A row of up to 1024 elements in 16 bits is one wave's (two chunks a lane), so its statistics need no barrier; narrower rows
+// share a wave, wider ones take 4 or 16.  Measured, 16384 rows of 1024 in bf16: forward 18.6 us (67 MB, 3.6 TB/s), backward
+// 22.4 us (101 MB, 4.5 TB/s) + 4.0 us for the parameter gradients' partial rows (1024 of them; 512 were 26.4 + 4.7).  4099
+// rows of 777 in fp32: 9.5, and 10.2 + 3.6 us.  16 rows of 512: 2.7 us.  (A forward kernel whose blocks
+// walk several rows, the next row and the weights asked for early, took 18.9 us.)
 #include "tokens.h"
 
 // A group of LPR lanes (up to 64), or of WPR whole waves, owns a row.

@@ -3,6 +3,9 @@
 // HBM-bound: every element is read and written once.  The angles are formed once per (token, pair) for all heads, in 64
 // bits - a 32-bit product of a far position and a frequency of 1 is off by 2^-24 of the position, in radians - reduced to
 // a part of a turn and passed on as 32-bit cosines and sines through LDS.  The backward pass is the turn by -t.
+// Measured, 65536 tokens of 16 x 64 channels in bf16: 45 us for 269 MB (6.0 TB/s: part of it stays in the last cache; a copy
+// of 256 MB runs at 5.4).  With one chunk in flight per thread, 64-bit divisions and the table read by elements it took 86.
+// 64 tokens of 32 x 128: 3.6 us.
 #include "tokens.h"
 
 #define ROT_MAX_PAIRS 256

@@ -15,6 +15,16 @@ template <> constexpr float xa_up<_Float16> = 7.f;
 // S^T = K Q^T leaves a row's scores in one lane pair, so the softmax runs in registers, and P^T is the B operand of
 // O^T += V^T P^T as it stands.  The running maximum is raised only when a score exceeds it by more than 2^8 (the
 // sums hold that in fp32): rescaling is rare after the first tile.
+//
+// Measured, 2 x 4096 rows over 4096 keys, 16 heads of 128 channels, bf16 (275 GFLOP): 262 to 277 us by card, 990 to 1050
+// TFLOP/s, where a matrix product of 8192 reaches 1320; the matrix pipes are busy 46 % of the cycles, LDS bank conflicts
+// are none.  Nothing bounds it alone: with four waves (287 us) the products by themselves took 140 us, with the softmax 177,
+// with the DMA 225, with the LDS reads 283 - two waves of a SIMD overlap one's products with the other's exponentials
+// only in part.  4 x 4096 rows over 657 to 1500 keys, 4 key heads of 64 channels (18 GFLOP): 34.8 us.  Measured and left out:
+// the next tile's scores under this tile's exponentials in one wave (305 us), a higher wave priority around the
+// products (287), one stage for V, three blocks per CU (they spill at 128 channels), reading fragments ahead (all within
+// 1 %).  With few blocks: four stages (16.4 against 13.8 us for 3 x 333 rows over 777 keys of 5 x 80), keys whole (23.4
+// against 13.7 + 5.4 for the join).
 // ---------------------------------------------------------------------------------------------------------------------
 template <int DP, int NW> struct XaFwd { static constexpr int STAGES = NW == 8 ? 3 : 2, LDS = STAGES * 2 * 64 * XaTile<DP>::RB; };
 template <typename T, int DP, int NW>
@@ -176,7 +186,9 @@ __global__ __launch_bounds__(64 * NW, 2) void xattn_fwd_kernel(XaArgs A) {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Few rows (up to 32 per key head: single tokens): the four waves of a block take turns at tiles of 32 keys of the block's
-// share of the keys, each with two DMA stages of its own (no barrier in the loop), and are joined through LDS.
+// share of the keys, each with two DMA stages of its own (no barrier in the loop), and are joined through LDS.  Bound by the
+// keys' and values' bytes: 16 x 1 token over 1072 to 4096 keys, 8 key heads for 32 of 128 channels, 174 MB: 40.7 us
+// (4.3 TB/s) + 4.9 for the join.  (Shares for 512 or 1024 blocks instead of 256: 44.1 and 48.4 us in all against 44.9.)
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 1) void xattn_token_kernel(XaArgs A) {
@@ -339,7 +351,8 @@ __global__ __launch_bounds__(256, 1) void xattn_token_kernel(XaArgs A) {
   }
 }
 
-// joins the shares of the keys: a wave per row.  The shares' weights are formed by one lane each (up to 64 shares); 16 lanes
+// joins the shares of the keys: a wave per row (a thread per 8 channels of a row took 26 us for 64 shares of one row, this
+// 4.7).  The shares' weights are formed by one lane each (up to 64 shares); 16 lanes
 // by 8 channels take every fourth share each, so a row's loads are in flight together, and the four sums are added.
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs A) {

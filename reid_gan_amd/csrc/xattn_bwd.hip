@@ -19,6 +19,34 @@ template <typename T> __device__ __forceinline__ u32x4 xa_rest(const f32x16& s, 
   return xa_as_b<T>(r, 0);
 }
 
+// s = A f^T and dp = B g^T over 32 rows of two tiles.  The fragments of AHEAD times 16 channels are asked for before their first
+// product: left to itself the compiler reads one, waits for it and multiplies (dk and dv of 2 x 16 heads of 128 channels, 2048
+// rows by 2048 keys: 263 -> 241 us; of 64 channels, the sizes below: 61 -> 58.5.  dq, with two waves per SIMD: 45 -> 44).
+template <typename T, int DP, int AHEAD>
+__device__ __forceinline__ void xa_scores(const char* a, const char* b, int row, int lane, const u32x4 (&f)[XaTile<DP>::KS],
+                                          const u32x4 (&g)[XaTile<DP>::KS], f32x16& s, f32x16& dp) {
+  constexpr int KS = XaTile<DP>::KS;
+  s = xa_zero();
+  dp = xa_zero();
+#pragma unroll
+  for (int k0 = 0; k0 < KS; k0 += AHEAD) {
+    u32x4 x[AHEAD], y[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (k0 + i < KS) {
+        x[i] = xa_frag<DP>(a, row, k0 + i, lane);
+        y[i] = xa_frag<DP>(b, row, k0 + i, lane);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (k0 + i < KS) {
+        s = xa_mma<T>(x[i], f[k0 + i], s);
+        dp = xa_mma<T>(y[i], g[k0 + i], dp);
+      }
+  }
+}
+
 // fp16 products hold dS only between 2^-24 and 2^16 while P alone spans more: dS travels times a power of two, lowered
 // (and the sums with it) when a value would pass 2^15.  bf16 has fp32's range and needs none.
 template <typename T> struct XaRange {
@@ -144,12 +172,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
         const char* vt = kt + TILE;
         auto keys32 = [&](auto u_) {
           constexpr int u = decltype(u_)::value;
-          f32x16 s = xa_zero(), dp = xa_zero();
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            s = xa_mma<T>(xa_frag<DP>(kt, 32 * u, ks, lane), fq[ks], s);
-            dp = xa_mma<T>(xa_frag<DP>(vt, 32 * u, ks, lane), fg[ks], dp);
-          }
+          f32x16 s, dp;
+          xa_scores<T, DP, 2>(kt, vt, 32 * u, lane, fq, fg, s, dp);
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = xa_exp2(__builtin_fmaf(s[r], c, -lse2));
           if (w != ~0ull) {                                       // (a hidden key's score reads as 0, not as nothing)
@@ -256,7 +280,9 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
 // takes one 64 keys with all rows, or the count is dealt out in even shares, one for every block that the chip holds: a share
 // begins and ends in the middle of some 64 keys' rows, and leaves those two as partial sums that the next kernel adds, in
 // the order of the shares.  With ragged lengths only the 64s that hold keys are counted.  Measured, the sizes above (36 GFLOP):
-// 60.5 us, 600 TFLOP/s, + 7.7 for the parts.  (Three blocks per CU, 32 rows a group: the registers spill, 88 us.)
+// 58.5 us, 620 TFLOP/s, + 7.7 for the parts.  (Three blocks per CU, 32 rows a group: the registers spill, 88 us.)  128
+// channels, 2 x 16 heads, 2048 rows by 2048 keys (137 GFLOP): 241 us, 570 TFLOP/s: a wave alone on its SIMD runs products
+// and the rest one after the other.  (The second 32 rows' scores before the first's exponentials: 250.)
 // ---------------------------------------------------------------------------------------------------------------------
 template <int DP>
 struct XaKv {
@@ -426,12 +452,8 @@ __global__ __launch_bounds__(64 * XaKv<DP>::NW, XaKv<DP>::BLOCKS) void xattn_dkv
         const float* rowv = reinterpret_cast<const float*>(smem + buf * STAGE + 2 * TILE) + grp * 64;
         auto rows32 = [&](auto u_) {
           constexpr int u = decltype(u_)::value;
-          f32x16 s = xa_zero(), dp = xa_zero();
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            s = xa_mma<T>(xa_frag<DP>(qt, 32 * u, ks, lane), fk[ks], s);
-            dp = xa_mma<T>(xa_frag<DP>(gt, 32 * u, ks, lane), fv[ks], dp);
-          }
+          f32x16 s, dp;
+          xa_scores<T, DP, KS>(qt, gt, 32 * u, lane, fk, fv, s, dp);
           float mx = 0.f;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {

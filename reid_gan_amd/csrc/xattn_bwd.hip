@@ -21,7 +21,7 @@ template <typename T> __device__ __forceinline__ u32x4 xa_rest(const f32x16& s, 
 
 // s = A f^T and dp = B g^T over 32 rows of two tiles.  The fragments of AHEAD times 16 channels are asked for before their first
 // product: left to itself the compiler reads one, waits for it and multiplies (dk and dv of 2 x 16 heads of 128 channels, 2048
-// rows by 2048 keys: 263 -> 241 us; of 64 channels, the sizes below: 61 -> 58.5.  dq, with two waves per SIMD: 45 -> 44).
+// rows by 2048 keys: 263 -> 241 us; of 64 channels, the sizes below: 61 -> 58.5).
 template <typename T, int DP, int AHEAD>
 __device__ __forceinline__ void xa_scores(const char* a, const char* b, int row, int lane, const u32x4 (&f)[XaTile<DP>::KS],
                                           const u32x4 (&g)[XaTile<DP>::KS], f32x16& s, f32x16& dp) {
@@ -71,7 +71,7 @@ __device__ __forceinline__ void xa_fit(float mx, float& es, f32x16 (&acc)[DT]) {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // dq: the forward kernel's tiling.  S^T = K Q^T and dP^T = V dO^T per 32 keys, dS^T is the B operand of dq^T += K^T dS^T.
-// Measured, 4 x 4096 rows over 657 to 1500 keys, 4 key heads of 64 channels (27 GFLOP): 42.2 us, 640 TFLOP/s; the matrix pipes
+// Measured, 4 x 4096 rows over 657 to 1500 keys, 4 key heads of 64 channels (27 GFLOP): 40.4 us, 670 TFLOP/s; the matrix pipes
 // are busy a quarter of the cycles.
 // Also leaves for the other kernel what its exponents add (p_up - lse, in powers of two; -infinity for a row without keys)
 // and Dl.
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
 // takes one 64 keys with all rows, or the count is dealt out in even shares, one for every block that the chip holds: a share
 // begins and ends in the middle of some 64 keys' rows, and leaves those two as partial sums that the next kernel adds, in
 // the order of the shares.  With ragged lengths only the 64s that hold keys are counted.  Measured, the sizes above (36 GFLOP):
-// 58.5 us, 620 TFLOP/s, + 7.7 for the parts.  (Three blocks per CU, 32 rows a group: the registers spill, 88 us.)  128
+// 57.1 us, 635 TFLOP/s, + 7.6 for the parts.  (Three blocks per CU, 32 rows a group: the registers spill, 88 us.)  128
 // channels, 2 x 16 heads, 2048 rows by 2048 keys (137 GFLOP): 241 us, 570 TFLOP/s: a wave alone on its SIMD runs products
 // and the rest one after the other.  (The second 32 rows' scores before the first's exponentials: 250.)
 // ---------------------------------------------------------------------------------------------------------------------

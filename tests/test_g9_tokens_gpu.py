@@ -626,6 +626,40 @@ def test_captured_forward_and_backward():
         assert all(torch.equal(a, t) for a, t in zip(got, results)), i
 
 
+@pytest.mark.parametrize("Lq, Lk", [(1000, 700), (2, 1500), (300, 130)])
+def test_captured_lengths_are_read_at_the_replay(Lq, Lk):
+    """A replay takes the lengths and the mask as they are then - also those that leave an entry, or all, without keys."""
+    B, H, Hk, D = 4, 8, 2, 64
+    g = gen(98)
+    q, k, v = qkv(99, B, Lq, Lk, H, Hk, D, BF16)
+    dout, lengths = normal(g, B, Lq, H, D, to=BF16), torch.full((B,), Lk, dtype=torch.int32, device=DEV)
+    mask = torch.ones(B, Lk, dtype=torch.bool, device=DEV)
+    out, dq, dk, dv = (torch.empty_like(t) for t in (q, q, k, v))
+    lse = torch.empty(B, H, Lq, device=DEV)
+    s1 = torch.empty(max(1, ops.xattn_fwd_scratch_floats(B, Lq, Lk, H, Hk, D)), device=DEV)
+    s2 = torch.empty(ops.xattn_bwd_scratch_floats(B, Lq, Lk, H, Hk, D), device=DEV)
+
+    def step():
+        ops.xattn_fwd(q, k, v, out, lse, 0.125, lengths, mask, s1)
+        ops.xattn_bwd(dout, q, k, v, out, lse, dq, dk, dv, 0.125, s2, lengths, mask)
+    step()
+    torch.cuda.synchronize()
+    graph = new_graph()
+    with torch.cuda.graph(graph):
+        step()
+    for lens in ([Lk, 1, Lk // 2, 65], [0, 0, 0, 0], [0, Lk, 0, 33], [-5, Lk + 9, 64, 2]):
+        lengths.copy_(torch.tensor(lens, dtype=torch.int32))
+        mask.copy_(torch.rand(B, Lk, generator=g, device=DEV) < 0.7)
+        for t in (out, dq, dk, dv, s1, s2):
+            t.fill_(7.0)
+        graph.replay()
+        leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+        want = attention.cross_attention(*leaves, lengths, mask, 0.125)
+        grads = torch.autograd.grad(want, leaves, dout)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((out, dq, dk, dv), (want, *grads))), lens
+
+
 def test_gradients_under_capture_are_refused():
     q, k, v = qkv(31, 1, 4, 8, 2, 2, 64, BF16)
     graph, kept = new_graph(), []

@@ -28,15 +28,17 @@ class _Bank:
         self.params, self.bits = params, bits
         self.dtype, self.device = params[0].dtype, params[0].device
         self.sizes = [p.numel() for p in params]
-        self.starts, blocks, first, pairs = [], 0, [0], []
-        for i, n in enumerate(self.sizes):
+        self.starts, blocks, first = [], 0, [0]
+        for n in self.sizes:
             self.starts.append(blocks * BLOCK)
             blocks += -(-n // BLOCK)
-            pairs.extend((i, c) for c in range(-(-n // CHUNK)))
-            first.append(len(pairs))
+            first.append(first[-1] + -(-n // CHUNK))
         self.first = array("i", first)
+        begin = torch.tensor(first)
+        tensor = torch.repeat_interleave(torch.arange(len(params)), begin.diff())
+        chunks = torch.stack((tensor, torch.arange(first[-1]) - begin[tensor]), 1)          # of a workgroup: (tensor, chunk of it)
         with torch.cuda.device(self.device):
-            self.map = torch.tensor(pairs or [(0, 0)], dtype=torch.int32, device=self.device)
+            self.map = (chunks if first[-1] else torch.zeros(1, 2)).to(torch.int32).to(self.device)
             self.steps = torch.zeros(len(params), dtype=torch.int32, device=self.device)
             self.coef = torch.zeros(len(params), 2, dtype=F32, device=self.device)
             many = max(blocks, 1) * BLOCK
@@ -53,15 +55,18 @@ class _Bank:
         self.elements = array("q", self.sizes)
         self.grads = array("q", bytes(8 * len(params)))
 
-    def views(self, i: int) -> Dict[str, torch.Tensor]:
-        """The state of tensor i, as views of the flat buffers."""
-        start, n, shape = self.starts[i], self.sizes[i], self.params[i].shape
-        out = {"step": self.steps[i]}
+    def views(self) -> List[Dict[str, torch.Tensor]]:
+        """The state of each tensor, as views of the flat buffers."""
+        blocks = [-(-n // BLOCK) for n in self.sizes]
+        pieces = [m for n, b in zip(self.sizes, blocks) for m in (n, b * BLOCK - n)]        # tensors and what lies between
+        out = [{"step": t} for t in self.steps.unbind()]
         for name, buf in self.flat.items():
             if name.endswith("_scale"):
-                out[name] = buf[start // BLOCK:start // BLOCK + -(-n // BLOCK)]
+                parts = buf[:sum(blocks)].split(blocks)
             else:
-                out[name] = buf[start:start + n].view(shape)
+                parts = [t.view(p.shape) for t, p in zip(buf[:sum(pieces)].split(pieces)[::2], self.params)]
+            for state, t in zip(out, parts):
+                state[name] = t
         return out
 
     def bind(self, at):
@@ -171,8 +176,8 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW: run a step before the capture")
         banks = self._banks[gi] = [_Bank(ps, group["state_bits"]) for ps in kinds.values()]
         for bank in banks:
-            for i, p in enumerate(bank.params):
-                saved, views = self.state.get(p), bank.views(i)
+            for p, views in zip(bank.params, bank.views()):
+                saved = self.state.get(p)
                 if saved:
                     self._take(saved, views)
                 self.state[p] = views

@@ -16,7 +16,7 @@ template <> constexpr float xa_up<_Float16> = 7.f;
 // O^T += V^T P^T as it stands.  The running maximum is raised only when a score exceeds it by more than 2^8 (the
 // sums hold that in fp32): rescaling is rare after the first tile.
 //
-// Measured, 2 x 4096 rows over 4096 keys, 16 heads of 128 channels, bf16 (275 GFLOP): 262 to 277 us by card, 990 to 1050
+// Measured, 2 x 4096 rows over 4096 keys, 16 heads of 128 channels, bf16 (275 GFLOP): 262 to 283 us by card, 970 to 1050
 // TFLOP/s, where a matrix product of 8192 reaches 1320; the matrix pipes are busy 46 % of the cycles, LDS bank conflicts
 // are none.  Nothing bounds it alone: with four waves (287 us) the products by themselves took 140 us, with the softmax 177,
 // with the DMA 225, with the LDS reads 283 - two waves of a SIMD overlap one's products with the other's exponentials

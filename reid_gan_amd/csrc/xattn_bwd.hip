@@ -19,7 +19,7 @@ template <typename T> __device__ __forceinline__ u32x4 xa_rest(const f32x16& s, 
   return xa_as_b<T>(r, 0);
 }
 
-// s = A f^T and dp = B g^T over 32 rows of two tiles.  The fragments of AHEAD times 16 channels are asked for before their first
+// s = A f^T and dp += B g^T over 32 rows of two tiles.  The fragments of AHEAD times 16 channels are asked for before their first
 // product: left to itself the compiler reads one, waits for it and multiplies (dk and dv of 2 x 16 heads of 128 channels, 2048
 // rows by 2048 keys: 263 -> 241 us; of 64 channels, the sizes below: 61 -> 58.5).
 template <typename T, int DP, int AHEAD>
@@ -27,7 +27,6 @@ __device__ __forceinline__ void xa_scores(const char* a, const char* b, int row,
                                           const u32x4 (&g)[XaTile<DP>::KS], f32x16& s, f32x16& dp) {
   constexpr int KS = XaTile<DP>::KS;
   s = xa_zero();
-  dp = xa_zero();
 #pragma unroll
   for (int k0 = 0; k0 < KS; k0 += AHEAD) {
     u32x4 x[AHEAD], y[AHEAD];
@@ -71,7 +70,7 @@ __device__ __forceinline__ void xa_fit(float mx, float& es, f32x16 (&acc)[DT]) {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // dq: the forward kernel's tiling.  S^T = K Q^T and dP^T = V dO^T per 32 keys, dS^T is the B operand of dq^T += K^T dS^T.
-// Measured, 4 x 4096 rows over 657 to 1500 keys, 4 key heads of 64 channels (27 GFLOP): 40.4 us, 670 TFLOP/s; the matrix pipes
+// Measured, 4 x 4096 rows over 657 to 1500 keys, 4 key heads of 64 channels (27 GFLOP): 39.4 us, 690 TFLOP/s; the matrix pipes
 // are busy a quarter of the cycles.
 // Also leaves for the other kernel what its exponents add (p_up - lse, in powers of two; -infinity for a row without keys)
 // and Dl.
@@ -149,7 +148,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
   const float c = A.scale * XA_LOG2E;
   XaTr<DP> tr(smem, lane);
   // tiles f .. e - 1 through the two stages, `use` on each 32 keys of a tile
-  auto sweep = [&](int f, int e, auto use) {
+  auto sweep = [&](int f, int e, const f32x16& start, auto use) {
     u64 w = 0;
     int byte = 0, buf = 0;
     if (f < e) {
@@ -172,7 +171,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
         const char* vt = kt + TILE;
         auto keys32 = [&](auto u_) {
           constexpr int u = decltype(u_)::value;
-          f32x16 s, dp;
+          f32x16 s, dp = start;
           xa_scores<T, DP, 2>(kt, vt, 32 * u, lane, fq, fg, s, dp);
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = xa_exp2(__builtin_fmaf(s[r], c, -lse2));
@@ -192,7 +191,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
     tr.move(buf ? -2 * TILE : 0);
   };
   if (few) {
-    sweep(0, ntile, [&](auto, f32x16& p, f32x16& dp) {
+    sweep(0, ntile, xa_zero(), [&](auto, f32x16& p, f32x16& dp) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) delta += p[r] * dp[r];
     });
@@ -204,19 +203,27 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
   }
   if (live && split == 0 && h == 0) {
     A.lse2[flat] = XaRange<T>::p_up - lse2;
-    A.delta[flat] = delta;
+    A.delta[flat] = -delta;
+  }
+  // up to 96 channels the registers hold -Dl as the products' first sum (44.0 -> 42.3 us for the sizes above on one card); above,
+  // it is subtracted after them
+  constexpr bool FOLD = DP <= 96;
+  f32x16 start = xa_zero();
+  if constexpr (FOLD) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) start[r] = -delta;
   }
   float es = XaRange<T>::on ? 0x1p24f : 1.f;
   f32x16 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = xa_zero();
   auto rows = [&](auto few_) {
-    sweep(t0, t1, [&](auto u_, f32x16& s, f32x16& dp) {
+    sweep(t0, t1, start, [&](auto u_, f32x16& s, f32x16& dp) {
       constexpr int u = decltype(u_)::value;
       float mx = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[r] *= dp[r] - delta;
+        s[r] *= FOLD ? dp[r] : dp[r] - delta;
         if constexpr (XaRange<T>::on) mx = fmaxf(mx, fabsf(s[r]));
       }
       if constexpr (XaRange<T>::on) {
@@ -280,7 +287,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XaArgs A) {
 // takes one 64 keys with all rows, or the count is dealt out in even shares, one for every block that the chip holds: a share
 // begins and ends in the middle of some 64 keys' rows, and leaves those two as partial sums that the next kernel adds, in
 // the order of the shares.  With ragged lengths only the 64s that hold keys are counted.  Measured, the sizes above (36 GFLOP):
-// 57.1 us, 635 TFLOP/s, + 7.6 for the parts.  (Three blocks per CU, 32 rows a group: the registers spill, 88 us.)  128
+// 56.4 us, 640 TFLOP/s, + 7.8 for the parts.  (Three blocks per CU, 32 rows a group: the registers spill, 88 us.)  128
 // channels, 2 x 16 heads, 2048 rows by 2048 keys (137 GFLOP): 241 us, 570 TFLOP/s: a wave alone on its SIMD runs products
 // and the rest one after the other.  (The second 32 rows' scores before the first's exponentials: 250.)
 // ---------------------------------------------------------------------------------------------------------------------
@@ -452,18 +459,23 @@ __global__ __launch_bounds__(64 * XaKv<DP>::NW, XaKv<DP>::BLOCKS) void xattn_dkv
         const float* rowv = reinterpret_cast<const float*>(smem + buf * STAGE + 2 * TILE) + grp * 64;
         auto rows32 = [&](auto u_) {
           constexpr int u = decltype(u_)::value;
-          f32x16 s, dp;
+          f32x16 s, dp;                                             // (dP - Dl: the sums begin at -Dl)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 d4 = *reinterpret_cast<const f32x4*>(rowv + ROWS + 32 * u + 8 * q + 4 * h);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dp[4 * q + i] = d4[i];
+          }
           xa_scores<T, DP, KS>(qt, gt, 32 * u, lane, fk, fv, s, dp);
           float mx = 0.f;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const f32x4 l4 = *reinterpret_cast<const f32x4*>(rowv + 32 * u + 8 * q + 4 * h);
-            const f32x4 d4 = *reinterpret_cast<const f32x4*>(rowv + ROWS + 32 * u + 8 * q + 4 * h);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int r = 4 * q + i;
               s[r] = xa_exp2(__builtin_fmaf(s[r], c, l4[i]));
-              dp[r] = s[r] * (dp[r] - d4[i]);
+              dp[r] *= s[r];
               if constexpr (XaRange<T>::on) mx = fmaxf(mx, fabsf(dp[r]));
             }
           }

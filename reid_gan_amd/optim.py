@@ -6,7 +6,8 @@ tensors, as on the drop-in module route; the fused TrainStep has its own update 
 from __future__ import annotations
 
 from array import array
-from typing import Dict, List
+from operator import is_
+from typing import Dict, List, Tuple
 
 import torch
 
@@ -145,7 +146,7 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
         for group in self.param_groups:
             self._check_values(group["lr"], group["betas"], group["eps"], group["weight_decay"])
-        self._banks: Dict[int, List[_Bank]] = {}
+        self._banks: Dict[int, Tuple[List[torch.Tensor], List[_Bank]]] = {}      # of a group: its parameters and their banks
 
     @staticmethod
     def _check_values(lr, betas, eps, weight_decay):
@@ -159,11 +160,13 @@ class AdamW(torch.optim.Optimizer):
         self._banks = {}
 
     def _group_banks(self, gi: int, group) -> List[_Bank]:
-        banks = self._banks.get(gi)
-        if banks is not None and sum(len(b.params) for b in banks) == len(group["params"]):
+        if gi in self._banks:
+            known, banks = self._banks[gi]
+            if len(known) != len(group["params"]) or not all(map(is_, known, group["params"])):
+                if len(known) != len(group["params"]) or set(map(id, known)) != set(map(id, group["params"])):
+                    raise RuntimeError("AdamW: a group's parameters changed after its first step; use add_param_group")
+                self._banks[gi] = list(group["params"]), banks              # (the same ones in another order)
             return banks
-        if banks is not None:
-            raise RuntimeError("AdamW: a group's parameters changed after its first step; use add_param_group")
         if len({id(p) for p in group["params"]}) != len(group["params"]):
             raise ValueError("AdamW: the same parameter twice in one group")
         if group["state_bits"] not in (32, 8):
@@ -174,7 +177,8 @@ class AdamW(torch.optim.Optimizer):
             kinds.setdefault((p.dtype, p.device), []).append(p)
         if kinds and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: run a step before the capture")
-        banks = self._banks[gi] = [_Bank(ps, group["state_bits"]) for ps in kinds.values()]
+        banks = [_Bank(ps, group["state_bits"]) for ps in kinds.values()]
+        self._banks[gi] = list(group["params"]), banks
         for bank in banks:
             for p, views in zip(bank.params, bank.views()):
                 saved = self.state.get(p)

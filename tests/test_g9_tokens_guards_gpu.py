@@ -1,0 +1,67 @@
+"""Calls of the token operators that have to be refused, or that must not lose anything: each of these once gave a wrong
+result, or grew, in silence."""
+import copy
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+pytestmark = pytest.mark.gpu
+
+from reid_gan_amd import attention, optim, rinet
+
+DEV = "cuda"
+BF16, F32 = torch.bfloat16, torch.float32
+GRAPHS = []            # captured graphs stay until the process ends
+SECTIONS = (8, 12, 12)
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def normal(seed, *shape, to=F32):
+    return torch.randn(*shape, generator=gen(seed), device=DEV).to(to)
+
+
+class Sub(torch.Tensor):
+    """A subclass keeps a call from going straight to the kernels: the checks in Python see it."""
+
+
+def calls():
+    """name, function of its tensors, the tensors"""
+    x, w, b = normal(1, 5, 64), normal(2, 64), normal(3, 64)
+    r, pos, freqs = normal(4, 1, 3, 2, 64), normal(5, 1, 3, 3), attention.rotary_frequencies(SECTIONS)
+    q, k, v = normal(6, 1, 3, 2, 64, to=BF16), normal(7, 1, 9, 2, 64, to=BF16), normal(8, 1, 9, 2, 64, to=BF16)
+    return {"layer_norm": (attention.layer_norm, (x, w, b)),
+            "rotary": (lambda t, p, f: attention.rotary(t, p, f, SECTIONS), (r, pos, freqs)),
+            "cross_attention": (attention.cross_attention, (q, k, v))}
+
+
+# --------------------------------------------------------------------------- AdamW: the group's parameters
+def ones(n):
+    p = torch.nn.Parameter(torch.ones(n, device=DEV))
+    p.grad = torch.ones(n, device=DEV)
+    return p
+
+
+def test_adamw_refuses_parameters_that_were_replaced():
+    a, b, new = ones(300), ones(7), ones(300)
+    opt = optim.AdamW([a, b])
+    opt.step()
+    before = [t.detach().clone() for t in (a, b, new)]
+    for params in ([new, b], [a, new], [b, new]):
+        opt.param_groups[0]["params"] = params
+        with pytest.raises(RuntimeError, match="add_param_group"):
+            opt.step()
+        with pytest.raises(RuntimeError, match="add_param_group"):
+            opt.flat_state()
+    opt.param_groups[0]["params"] = [a, b]
+    opt.param_groups[0]["params"][0] = new                                  # in the list itself
+    with pytest.raises(RuntimeError, match="add_param_group"):
+        opt.step()
+    assert all(torch.equal(t, o) for t, o in zip((a, b, new), before))
+    opt.param_groups[0]["params"] = [b, a]                                  # the same ones in another order
+    opt.step()
+    assert not torch.equal(a, before[0]) and not torch.equal(b, before[1])
+    assert int(opt.state[a]["step"]) == int(opt.state[b]["step"]) == 2

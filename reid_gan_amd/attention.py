@@ -9,10 +9,10 @@ Tensors live on a ROCm device (there is no CPU path) in fp32, bf16 or fp16 (cros
 statistics and softmax are fp32 whatever the type.  Every call runs on the current stream of its tensors' device and
 allocates what it needs from torch's allocator, so calls on different streams share nothing.
 
-The functions here are differentiable, but their gradients are not made for graph capture: torch's AccumulateGrad nodes
-remember the stream of an earlier eager pass, and a captured backward that meets one ends the process.  A captured
-step calls the forward and backward functions of reid_gan_amd.ops on buffers of its own (as TrainStep does); without
-gradients the functions here may be captured as they are.
+The functions here are differentiable backwards, once; tensors with a forward-mode tangent are refused.  Their gradients are
+not made for graph capture: torch's AccumulateGrad nodes remember the stream of an earlier eager pass, and a captured
+backward that meets one ends the process.  A captured step calls the forward and backward functions of reid_gan_amd.ops
+on buffers of its own (as TrainStep does); without gradients the functions here may be captured as they are.
 """
 from __future__ import annotations
 
@@ -47,6 +47,11 @@ def _on_gpu(what: str, t: torch.Tensor):
         raise RuntimeError(f"{what}: tensors must be on a ROCm device; there is no CPU path")
 
 
+def _check_derivatives(what: str, *tensors):
+    if direct().dual(*tensors):
+        raise RuntimeError(f"{what}: there is no forward-mode derivative, and a tensor has a tangent (take it off with unpack_dual)")
+
+
 def _not_captured(what: str):
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{what}: gradients are not taken under graph capture; capture the forward and backward "
@@ -59,6 +64,7 @@ def _once(backward):
     guarded = once_differentiable(backward)
 
     def run(ctx, grad):
+        _check_derivatives("backward", grad)
         return guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
     return run
 
@@ -132,6 +138,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     y = direct().layer_norm(x, weight, bias, eps)
     if y is not None:
         return y
+    _check_derivatives("layer_norm", x, weight, bias)
     _check_layer_norm(x, weight, bias, eps)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
@@ -211,6 +218,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sectio
         y = direct().rotary(x, positions, freqs, sections, interleaved, inverse)
         if y is not None:
             return y
+    _check_derivatives("rotary", x, positions, freqs, out)
     _check_tensor("rotary", "x", x, ops.TOKEN_TYPES)
     if x.dim() != 4:
         raise ValueError("rotary: x is [batch][tokens][heads][channels]")
@@ -312,6 +320,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: 
     o = direct().cross_attention(q, k, v, lengths, key_mask, scale)
     if o is not None:
         return o
+    _check_derivatives("cross_attention", q, k, v)
     _check_tensor("cross_attention", "q", q, _CROSS_TYPES)
     device, kind = q.device, (q.dtype,)
     _check_tensor("cross_attention", "k", k, kind, device)

@@ -54,6 +54,12 @@ void check(const char* what, int rc) { TORCH_CHECK(rc == 0, what, " failed (", r
 void not_captured(const char* what, const Tensor& t) {
   TORCH_CHECK(!capturing(t), what, ": gradients are not taken under graph capture; capture the forward and backward functions of reid_gan_amd.ops instead");
 }
+// A tensor with a forward-mode tangent: the kernels have no derivative in that direction, and a result without a tangent would
+// stand for a derivative of zero.
+bool dual(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+void one_way(const char* what, const Tensor& grad) {
+  TORCH_CHECK(!dual(grad), what, ": there is no forward-mode derivative of its gradients, and the incoming one has a tangent");
+}
 const void* address(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 Tensor floats(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
 Tensor fresh(const Tensor& like) { return at::empty(like.sizes(), like.options()); }
@@ -99,6 +105,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
     c10::DeviceGuard guard(x.device());
     not_captured("layer_norm", x);
+    one_way("layer_norm", grads[0]);
     Tensor dy = grads[0].contiguous();
     const int64_t C = x.size(-1), rows = x.numel() / C;
     Tensor dx = fresh(x), dw, db, scratch;
@@ -146,6 +153,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
     const variable_list saved = ctx->get_saved_variables();
     c10::DeviceGuard guard(grads[0].device());
     not_captured("rotary", grads[0]);
+    one_way("rotary", grads[0]);
     const std::vector<int64_t> v = ctx->saved_data["turn"].toIntVector();
     Turn t = {saved[0], saved[1]};
     for (int i = 0; i < 4; ++i) t.sections[i] = static_cast<int>(v[i]);
@@ -205,6 +213,7 @@ struct Cross : torch::autograd::Function<Cross> {
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &lse = saved[4];
     c10::DeviceGuard guard(q.device());
     not_captured("cross_attention", q);
+    one_way("cross_attention", grads[0]);
     Tensor dq = fresh(q), dk = fresh(k), dv = fresh(v);
     if (q.size(1) == 0) {
       dk.zero_();
@@ -262,6 +271,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
                          (t->scalar_type() != at::kFloat && t->scalar_type() != x.scalar_type())))
       Py_RETURN_NONE;
   if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type()) Py_RETURN_NONE;
+  if (dual(x) || dual(w) || dual(b)) Py_RETURN_NONE;
   c10::DeviceGuard guard(x.device());
   if (!wanted({&x, &w, &b})) return THPVariable_Wrap(layer_norm(x, w, b, eps, nullptr));
   if (capturing(x)) Py_RETURN_NONE;
@@ -299,6 +309,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   for (int i = 0; i < 4; ++i)
     if (x.size(i) > 0x7fffffff) Py_RETURN_NONE;
+  if (dual(x) || dual(pos) || dual(freqs)) Py_RETURN_NONE;
   t.pos = pos;
   t.freqs = freqs;
   c10::DeviceGuard guard(x.device());
@@ -331,10 +342,20 @@ PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   if (a[5] == Py_None) scale = 1.0 / std::sqrt(static_cast<double>(D));
   if (!(scale > 0 && scale < 1e30)) Py_RETURN_NONE;
+  if (dual(q) || dual(k) || dual(v)) Py_RETURN_NONE;
   c10::DeviceGuard guard(q.device());
   if (!wanted({&q, &k, &v})) return THPVariable_Wrap(attend(q, k, v, Tensor(), lengths, mask, scale));
   if (capturing(q)) Py_RETURN_NONE;
   return THPVariable_Wrap(Cross::apply(q, k, v, Keys{lengths, mask}, scale));
+  END_HANDLE_TH_ERRORS
+}
+
+// dual(*tensors): whether one of the arguments is a tensor with a forward-mode tangent
+PyObject* py_dual(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (THPVariable_Check(a[i]) && dual(THPVariable_Unpack(a[i]))) Py_RETURN_TRUE;
+  Py_RETURN_FALSE;
   END_HANDLE_TH_ERRORS
 }
 
@@ -409,6 +430,7 @@ PyMethodDef methods[] = {
     {"layer_norm", FAST(py_layer_norm), "layer_norm(x, weight, bias, eps), or None where more than the launch is needed"},
     {"rotary", FAST(py_rotary), "rotary(x, positions, freqs, sections, interleaved, inverse), or None"},
     {"cross_attention", FAST(py_cross_attention), "cross_attention(q, k, v, lengths, key_mask, scale), or None"},
+    {"dual", FAST(py_dual), "dual(*tensors): whether one of them has a forward-mode tangent"},
     {"gradients", FAST(py_gradients), "gradients(params, addresses, sizes, out): whether out holds the gradients' addresses"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", "Direct calls of the token operators", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -65,3 +65,24 @@ def test_adamw_refuses_parameters_that_were_replaced():
     opt.step()
     assert not torch.equal(a, before[0]) and not torch.equal(b, before[1])
     assert int(opt.state[a]["step"]) == int(opt.state[b]["step"]) == 2
+
+
+# --------------------------------------------------------------------------- derivatives and traces that would be lost
+@pytest.mark.parametrize("name", ["layer_norm", "rotary", "cross_attention"])
+@pytest.mark.parametrize("plain", [True, False])
+def test_forward_mode_derivatives_are_refused(name, plain):
+    call, args = calls()[name]
+    wrap = (lambda t: t) if plain else (lambda t: t.as_subclass(Sub))
+    with forward_ad.dual_level():
+        for i, t in enumerate(args):
+            dual = [forward_ad.make_dual(a, torch.ones_like(a)) if j == i else a for j, a in enumerate(args)]
+            for grad in (False, True):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*map(wrap, dual))
+        call(*map(wrap, args))                                              # (tensors without a tangent are none of its business)
+        with forward_ad._set_fwd_grad_enabled(False):
+            call(*map(wrap, dual))
+        leaf = args[0].detach().clone().requires_grad_()                    # and the incoming gradient of a backward pass
+        out = call(*map(wrap, (leaf, *args[1:])))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, leaf, forward_ad.make_dual(torch.ones_like(args[0]), torch.ones_like(args[0])))

@@ -1,0 +1,30 @@
+"""What the token operators refuse before any launch, because a result would lack something in silence; no GPU needed."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from reid_gan_amd import attention
+
+BF16 = torch.bfloat16
+
+
+def calls():
+    """name: function of its tensors, the tensors"""
+    x, w, b = torch.ones(5, 64), torch.ones(64), torch.zeros(64)
+    r, pos, freqs = torch.ones(1, 3, 2, 64), torch.ones(1, 3, 3), attention.rotary_frequencies((8, 12, 12), device="cpu")
+    q, k, v = (torch.ones(1, n, 2, 64, dtype=BF16) for n in (3, 9, 9))
+    return {"layer_norm": (attention.layer_norm, (x, w, b)),
+            "rotary": (lambda t, p, f: attention.rotary(t, p, f, (8, 12, 12)), (r, pos, freqs)),
+            "cross_attention": (attention.cross_attention, (q, k, v))}
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "rotary", "cross_attention"])
+def test_forward_mode_derivatives_are_refused(name):
+    call, args = calls()[name]
+    with forward_ad.dual_level():
+        for i in range(3):
+            dual = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(args)]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(*dual)
+        with pytest.raises(RuntimeError, match="no CPU path"):              # (no tangent: nothing to refuse but the device)
+            call(*args)

@@ -9,10 +9,11 @@ Tensors live on a ROCm device (there is no CPU path) in fp32, bf16 or fp16 (cros
 statistics and softmax are fp32 whatever the type.  Every call runs on the current stream of its tensors' device and
 allocates what it needs from torch's allocator, so calls on different streams share nothing.
 
-The functions here are differentiable backwards, once; tensors with a forward-mode tangent are refused.  Their gradients are
-not made for graph capture: torch's AccumulateGrad nodes remember the stream of an earlier eager pass, and a captured
-backward that meets one ends the process.  A captured step calls the forward and backward functions of reid_gan_amd.ops
-on buffers of its own (as TrainStep does); without gradients the functions here may be captured as they are.
+The functions here are differentiable backwards, once; tensors with a forward-mode tangent are refused, and so is a call
+under torch.jit.trace or make_fx.  Gradients are not made for graph capture: torch's AccumulateGrad nodes remember the
+stream of an earlier eager pass, and a captured backward that meets one ends the process.  A captured step calls the
+forward and backward functions of reid_gan_amd.ops on buffers of its own (as TrainStep does); without gradients the
+functions here may be captured as they are.
 """
 from __future__ import annotations
 
@@ -47,7 +48,10 @@ def _on_gpu(what: str, t: torch.Tensor):
         raise RuntimeError(f"{what}: tensors must be on a ROCm device; there is no CPU path")
 
 
-def _check_derivatives(what: str, *tensors):
+def _check_recording(what: str, *tensors):
+    if direct().traced():
+        raise RuntimeError(f"{what}: cannot be traced (the trace would hold the allocation of the result without the kernel that "
+                           "writes it)")
     if direct().dual(*tensors):
         raise RuntimeError(f"{what}: there is no forward-mode derivative, and a tensor has a tangent (take it off with unpack_dual)")
 
@@ -64,7 +68,7 @@ def _once(backward):
     guarded = once_differentiable(backward)
 
     def run(ctx, grad):
-        _check_derivatives("backward", grad)
+        _check_recording("backward", grad)
         return guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
     return run
 
@@ -138,7 +142,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     y = direct().layer_norm(x, weight, bias, eps)
     if y is not None:
         return y
-    _check_derivatives("layer_norm", x, weight, bias)
+    _check_recording("layer_norm", x, weight, bias)
     _check_layer_norm(x, weight, bias, eps)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
@@ -218,7 +222,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sectio
         y = direct().rotary(x, positions, freqs, sections, interleaved, inverse)
         if y is not None:
             return y
-    _check_derivatives("rotary", x, positions, freqs, out)
+    _check_recording("rotary", x, positions, freqs, out)
     _check_tensor("rotary", "x", x, ops.TOKEN_TYPES)
     if x.dim() != 4:
         raise ValueError("rotary: x is [batch][tokens][heads][channels]")
@@ -320,7 +324,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: 
     o = direct().cross_attention(q, k, v, lengths, key_mask, scale)
     if o is not None:
         return o
-    _check_derivatives("cross_attention", q, k, v)
+    _check_recording("cross_attention", q, k, v)
     _check_tensor("cross_attention", "q", q, _CROSS_TYPES)
     device, kind = q.device, (q.dtype,)
     _check_tensor("cross_attention", "k", k, kind, device)

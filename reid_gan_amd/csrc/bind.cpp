@@ -8,12 +8,14 @@
 // most).
 #include <Python.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/torch.h>
 
 #include "../../include/ried_gan.h"
@@ -53,6 +55,12 @@ bool capturing(const Tensor& t) {
 void check(const char* what, int rc) { TORCH_CHECK(rc == 0, what, " failed (", rc, "): ", abi.last_error()); }
 void not_captured(const char* what, const Tensor& t) {
   TORCH_CHECK(!capturing(t), what, ": gradients are not taken under graph capture; capture the forward and backward functions of reid_gan_amd.ops instead");
+}
+// Whether torch records the operations of this thread (jit.trace, make_fx): the recording would hold the allocation of a result
+// and not the kernel that writes it.
+bool traced() {
+  return torch::jit::tracer::isTracing() ||
+         c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
 }
 // A tensor with a forward-mode tangent: the kernels have no derivative in that direction, and a result without a tangent would
 // stand for a derivative of zero.
@@ -250,8 +258,8 @@ bool number(PyObject* o, double& v) {
   }
   return true;
 }
-// ready for a call: a ROCm tensor; where gradients are wanted, not under capture
-bool ready(const Tensor& t) { return connected && t.is_cuda(); }
+// ready for a call: a ROCm tensor, outside a trace
+bool ready(const Tensor& t) { return connected && t.is_cuda() && !traced(); }
 bool wanted(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
@@ -359,6 +367,13 @@ PyObject* py_dual(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* py_traced(PyObject*, PyObject*) {
+  HANDLE_TH_ERRORS
+  if (traced()) Py_RETURN_TRUE;
+  Py_RETURN_FALSE;
+  END_HANDLE_TH_ERRORS
+}
+
 // A buffer of int64 (array.array('q')), released at the end of its scope
 struct Words {
   Py_buffer view = {};
@@ -431,6 +446,7 @@ PyMethodDef methods[] = {
     {"rotary", FAST(py_rotary), "rotary(x, positions, freqs, sections, interleaved, inverse), or None"},
     {"cross_attention", FAST(py_cross_attention), "cross_attention(q, k, v, lengths, key_mask, scale), or None"},
     {"dual", FAST(py_dual), "dual(*tensors): whether one of them has a forward-mode tangent"},
+    {"traced", py_traced, METH_NOARGS, "traced(): whether torch records the operations of this thread"},
     {"gradients", FAST(py_gradients), "gradients(params, addresses, sizes, out): whether out holds the gradients' addresses"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", "Direct calls of the token operators", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -86,3 +86,24 @@ def test_forward_mode_derivatives_are_refused(name, plain):
         out = call(*map(wrap, (leaf, *args[1:])))
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(out, leaf, forward_ad.make_dual(torch.ones_like(args[0]), torch.ones_like(args[0])))
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "rotary", "cross_attention"])
+@pytest.mark.parametrize("plain", [True, False])
+def test_traces_are_refused(name, plain):
+    """A trace would hold the allocation of the result and not the kernel that writes it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, args = calls()[name]
+    wrap = (lambda t: t) if plain else (lambda t: t.as_subclass(Sub))
+    function = lambda *ts: call(*map(wrap, ts)).as_subclass(torch.Tensor)
+    want = function(*args)
+    for grad in (False, True):
+        leaves = [a.detach().requires_grad_(grad and i == 0) for i, a in enumerate(args)]
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(function, tuple(leaves), check_trace=False)
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(function)(*leaves)
+    assert torch.equal(function(*args), want)
+    if name == "layer_norm":
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(attention.LayerNorm(64).to(DEV), args[0], check_trace=False)

@@ -28,3 +28,15 @@ def test_forward_mode_derivatives_are_refused(name):
                 call(*dual)
         with pytest.raises(RuntimeError, match="no CPU path"):              # (no tangent: nothing to refuse but the device)
             call(*args)
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "rotary", "cross_attention"])
+def test_traces_are_refused(name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, args = calls()[name]
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(call, args, check_trace=False)
+    with pytest.raises(RuntimeError, match="traced"):
+        make_fx(lambda *ts: call(*ts))(*args)
+    with pytest.raises(RuntimeError, match="no CPU path"):                  # (outside a trace: nothing to refuse but the device)
+        call(*args)

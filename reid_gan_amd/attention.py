@@ -217,7 +217,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sectio
     between the decoder's).  sections: pairs of each axis (slice, row, column ...), one to four; freqs: fp64 table of
     rotary_frequencies, sum(sections) entries.  Pair j is channels (j, j + pairs), or (2j, 2j + 1) when interleaved;
     channels behind the pairs pass through.  Angles are formed in 64 bits, so far positions keep their precision.
-    inverse turns back (and is the gradient).  out: where to write, also x itself (no gradients then)."""
+    inverse turns back (and is the gradient, which x alone has: positions and freqs that require one are refused).  out: where
+    to write, also x itself (no gradients then)."""
     if out is None:
         y = direct().rotary(x, positions, freqs, sections, interleaved, inverse)
         if y is not None:
@@ -238,6 +239,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sectio
     _check_tensor("rotary", "freqs", freqs, (torch.float64,), x.device)
     if freqs.shape != (pairs,) or not freqs.is_contiguous():
         raise ValueError(f"rotary: freqs is a contiguous table of {pairs} entries")
+    if torch.is_grad_enabled() and (positions.requires_grad or freqs.requires_grad):
+        raise RuntimeError("rotary: positions and freqs have no gradient; pass them detached")
     adjacent = D == 1 or x.stride(3) == 1
     if out is None:
         _on_gpu("rotary", x)

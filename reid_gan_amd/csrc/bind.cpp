@@ -317,7 +317,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   for (int i = 0; i < 4; ++i)
     if (x.size(i) > 0x7fffffff) Py_RETURN_NONE;
-  if (dual(x) || dual(pos) || dual(freqs)) Py_RETURN_NONE;
+  if (dual(x) || dual(pos) || dual(freqs) || wanted({&pos, &freqs})) Py_RETURN_NONE;   // (the tables have no gradient)
   t.pos = pos;
   t.freqs = freqs;
   c10::DeviceGuard guard(x.device());

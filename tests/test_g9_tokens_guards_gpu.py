@@ -107,3 +107,18 @@ def test_traces_are_refused(name, plain):
     if name == "layer_norm":
         with pytest.raises(RuntimeError, match="traced"):
             torch.jit.trace(attention.LayerNorm(64).to(DEV), args[0], check_trace=False)
+
+
+@pytest.mark.parametrize("plain", [True, False])
+def test_rotary_refuses_gradients_of_its_tables(plain):
+    call, (x, pos, freqs) = calls()["rotary"]
+    wrap = (lambda t: t) if plain else (lambda t: t.as_subclass(Sub))
+    for leaf in (pos, freqs):
+        leaf.requires_grad_()
+        for first in (x, x.clone().requires_grad_()):
+            with pytest.raises(RuntimeError, match="positions and freqs have no gradient"):
+                call(wrap(first), pos, freqs)
+        with torch.no_grad():
+            got = call(wrap(x), pos, freqs)
+        leaf.requires_grad_(False)
+        assert torch.equal(got.as_subclass(torch.Tensor), call(x, pos, freqs))

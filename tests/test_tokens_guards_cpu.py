@@ -40,3 +40,14 @@ def test_traces_are_refused(name):
         make_fx(lambda *ts: call(*ts))(*args)
     with pytest.raises(RuntimeError, match="no CPU path"):                  # (outside a trace: nothing to refuse but the device)
         call(*args)
+
+
+def test_rotary_refuses_gradients_of_its_tables():
+    call, (x, pos, freqs) = calls()["rotary"]
+    for leaf in (pos, freqs):
+        leaf.requires_grad_()
+        with pytest.raises(RuntimeError, match="positions and freqs have no gradient"):
+            call(x, pos, freqs)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+            call(x, pos, freqs)
+        leaf.requires_grad_(False)

@@ -388,7 +388,7 @@ struct Words {
 };
 
 // gradients(params, addresses, sizes, out): out[i] = address of the i-th parameter's gradient (0: none).  False when a
-// parameter is not at its address any more, or a gradient is not a contiguous one of the parameter's type and size.
+// parameter does not lie at its address as it did, or a gradient is not a contiguous one of the parameter's type and size.
 // Parameters with a gradient count as written (an earlier graph that saved one must not use it any more).
 PyObject* py_gradients(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -400,7 +400,8 @@ PyObject* py_gradients(PyObject*, PyObject* const* a, Py_ssize_t n) {
     PyObject* o = PyList_GET_ITEM(a[0], i);
     if (!THPVariable_Check(o)) Py_RETURN_FALSE;
     const Tensor& p = THPVariable_Unpack(o);
-    if (reinterpret_cast<int64_t>(p.const_data_ptr()) != at.data()[i]) Py_RETURN_FALSE;
+    if (reinterpret_cast<int64_t>(p.const_data_ptr()) != at.data()[i] || p.numel() != sizes.data()[i] || !p.is_contiguous() || p.is_neg())
+      Py_RETURN_FALSE;
     const Tensor& g = p.grad();
     if (!g.defined()) {
       out.data()[i] = 0;

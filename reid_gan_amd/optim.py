@@ -96,8 +96,8 @@ class _Bank:
         if direct().gradients(self.params, self.at, self.elements, self.grads):
             return ()
         at = array("q", [p.data_ptr() for p in self.params])
-        if at != self.at:
-            self.bind(at)
+        if at != self.at or any(p.numel() != n or not p.is_contiguous() or p.is_neg() for p, n in zip(self.params, self.sizes)):
+            self.bind(at)                                         # (which refuses a parameter that lies there otherwise)
         kept = []
         for i, (p, n) in enumerate(zip(self.params, self.sizes)):
             g = p.grad

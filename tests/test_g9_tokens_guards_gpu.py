@@ -67,6 +67,21 @@ def test_adamw_refuses_parameters_that_were_replaced():
     assert int(opt.state[a]["step"]) == int(opt.state[b]["step"]) == 2
 
 
+def test_adamw_refuses_a_parameter_that_was_transposed_where_it_lies():
+    p = torch.nn.Parameter(normal(20, 16, 16))
+    opt = optim.AdamW([p])
+    p.grad = normal(21, 16, 16)
+    opt.step()
+    p.data = p.data.t()
+    p.grad = normal(21, 16, 16)
+    before = p.detach().clone()
+    with pytest.raises(ValueError, match="contiguous"):
+        opt.step()
+    assert torch.equal(p, before)
+    p.data = p.data.t()
+    opt.step()
+
+
 # --------------------------------------------------------------------------- derivatives and traces that would be lost
 @pytest.mark.parametrize("name", ["layer_norm", "rotary", "cross_attention"])
 @pytest.mark.parametrize("plain", [True, False])

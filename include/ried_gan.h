@@ -518,7 +518,7 @@ typedef struct ried_xattn {
   void *dq, *dk, *dv;
   long long q_stride[3], k_stride[3], v_stride[3], o_stride[3], dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
   long long mask_stride, batch, queries, keys, heads, groups, dim, type;
-  double scale;
+  double scale;                             /* between 1e-37 and 1e30 */
 } ried_xattn_t;
 long long ried_xattn_fwd_scratch_floats(long long batch, long long queries, long long keys, int heads, int groups, int dim);
 int ried_xattn_fwd(const ried_xattn_t* desc_host, ried_stream_t stream);

@@ -322,8 +322,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: 
     Head h reads key head h // (heads // key heads).  lengths: int32 [batch], the first so many keys of each entry
     count; key_mask: bool or uint8 [batch][keys], nonzero keys count; with both, keys that both allow.  An entry without
     keys gives zeros and no gradient; hidden keys have no effect whatever they hold, and get zero gradients.  scale:
-    channels ** -0.5 unless given.  channels: a multiple of 8 up to 128, bf16 or fp16.  Views are read where they lie when
-    their channels are adjacent and their strides are multiples of 8 elements; others are copied."""
+    channels ** -0.5 unless given (between 1e-37 and 1e30).  channels: a multiple of 8 up to 128, bf16 or fp16.  Views are
+    read where they lie when their channels are adjacent and their strides are multiples of 8 elements; others are copied."""
     o = direct().cross_attention(q, k, v, lengths, key_mask, scale)
     if o is not None:
         return o
@@ -352,8 +352,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: 
         if key_mask.stride(0) < 0 or (key_mask.stride(1) != 1 and key_mask.shape[1] > 1):
             key_mask = key_mask.contiguous()
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0 < scale < 1e30:
-        raise ValueError("cross_attention: scale is a positive number")
+    if not 1e-37 < scale < 1e30:
+        raise ValueError("cross_attention: scale is a positive number between 1e-37 and 1e30")
     _on_gpu("cross_attention", q)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _CrossFn.apply(q, k, v, lengths, key_mask, scale)

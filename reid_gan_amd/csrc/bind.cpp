@@ -349,7 +349,7 @@ PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                          (mask.stride(1) != 1 && mask.size(1) > 1)))
     Py_RETURN_NONE;
   if (a[5] == Py_None) scale = 1.0 / std::sqrt(static_cast<double>(D));
-  if (!(scale > 0 && scale < 1e30)) Py_RETURN_NONE;
+  if (!(scale > 1e-37 && scale < 1e30)) Py_RETURN_NONE;
   if (dual(q) || dual(k) || dual(v)) Py_RETURN_NONE;
   c10::DeviceGuard guard(q.device());
   if (!wanted({&q, &k, &v})) return THPVariable_Wrap(attend(q, k, v, Tensor(), lengths, mask, scale));

@@ -438,7 +438,8 @@ int xa_check(const ried_xattn_t* d, const char* name, bool bwd) {
   RIED_CHECK_ARG(d->keys <= (1ll << 30) && d->queries <= (1ll << 30) && d->batch <= (1ll << 20) && d->heads <= (1ll << 20) &&
                  d->heads / d->groups * d->queries <= (1ll << 30) && d->batch * d->groups <= (1ll << 24),
                  "%s: sizes out of range", name);
-  RIED_CHECK_ARG(d->scale > 0 && d->scale < 1e30, "%s: the scale is a positive number", name);
+  // (below, the kernels' factor would be zero in 32 bits, and zero times a hidden key's -infinity is not a number)
+  RIED_CHECK_ARG(d->scale > 1e-37 && d->scale < 1e30, "%s: the scale is a positive number between 1e-37 and 1e30", name);
   if (d->batch == 0 || d->queries == 0) return RIED_OK;
   struct View { const void* p; const long long* s; const char* n; bool need; } views[] = {
       {d->q, d->q_stride, "q", true}, {d->k, d->k_stride, "k", d->keys > 0}, {d->v, d->v_stride, "v", d->keys > 0},

@@ -137,3 +137,16 @@ def test_rotary_refuses_gradients_of_its_tables(plain):
             got = call(wrap(x), pos, freqs)
         leaf.requires_grad_(False)
         assert torch.equal(got.as_subclass(torch.Tensor), call(x, pos, freqs))
+
+
+def test_cross_attention_small_scales_keep_hidden_keys_out():
+    """A scale close to nothing: the result is the mean of the values that count."""
+    _, (q, k, v) = calls()["cross_attention"]
+    mask = torch.tensor([[True, False] * 4 + [True]], device=DEV)
+    want = v[:, ::2].double().mean(1, keepdim=True)
+    for rows in (3, 90):
+        got = attention.cross_attention(q.repeat(1, rows // 3, 1, 1), k, v, key_mask=mask, scale=2e-37)
+        assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -8 * v.double().abs().mean(1, keepdim=True)).all())
+    for scale in (1e-46, 1e30):
+        with pytest.raises(ValueError, match="scale"):
+            attention.cross_attention(q, k, v, key_mask=mask, scale=scale)

@@ -1,9 +1,11 @@
 """What the token operators refuse before any launch, because a result would lack something in silence; no GPU needed."""
+import struct
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from reid_gan_amd import attention
+from reid_gan_amd import _lib, attention
 
 BF16 = torch.bfloat16
 
@@ -51,3 +53,22 @@ def test_rotary_refuses_gradients_of_its_tables():
         with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
             call(x, pos, freqs)
         leaf.requires_grad_(False)
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e-38, 1e30])
+def test_cross_attention_refuses_scales_that_32_bits_lose(scale):
+    """A factor of zero would turn the -infinity of hidden keys into NaN, and with it whole rows."""
+    call, args = calls()["cross_attention"]
+    with pytest.raises(ValueError, match="scale"):
+        call(*args, scale=scale)
+    at, strides = 1 << 20, (64, 64, 64)                                     # (an address that nothing dereferences)
+    desc = struct.pack("=12q24q8qd", *(at,) * 5, 0, 0, *(at,) * 5, *strides * 8, 0, 1, 1, 1, 1, 1, 64, 1, scale)
+    for entry in (_lib.lib.ried_xattn_fwd, _lib.lib.ried_xattn_bwd):
+        with pytest.raises(RuntimeError, match="scale"):
+            entry(desc, None)
+
+
+def test_cross_attention_takes_small_scales():
+    call, args = calls()["cross_attention"]
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        call(*args, scale=1e-36)

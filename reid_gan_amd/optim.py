@@ -205,7 +205,13 @@ class AdamW(torch.optim.Optimizer):
         return [bank.flat for gi, group in enumerate(self.param_groups) for bank in self._group_banks(gi, group)]
 
     def load_state_dict(self, state_dict):
-        """Copies the saved moments into this optimizer's buffers (so a captured step goes on with them)."""
+        """Copies the saved moments into this optimizer's buffers (so a captured step goes on with them); registered hooks run
+        before and after."""
+        state_dict = dict(state_dict)                             # (a hook may change its own)
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            changed = hook(self, state_dict)
+            if changed is not None:
+                state_dict = changed
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("AdamW: the state dict has other parameter groups")
@@ -225,6 +231,8 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     for t in views.values():
                         (t.view(torch.uint8) if t.dtype is CODES else t).zero_()
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     @torch.no_grad()
     def step(self, closure=None):

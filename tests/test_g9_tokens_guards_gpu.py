@@ -82,6 +82,32 @@ def test_adamw_refuses_a_parameter_that_was_transposed_where_it_lies():
     opt.step()
 
 
+# --------------------------------------------------------------------------- AdamW: state dicts
+def test_adamw_load_state_dict_runs_its_hooks():
+    a, b = ones(5), ones(5)
+    one, two = optim.AdamW([a], lr=1e-3), optim.AdamW([b], lr=1e-3)
+    one.step()
+    seen = []
+
+    def before(opt, state):
+        seen.append("before")
+        state = copy.deepcopy(state)
+        state["param_groups"][0]["lr"] = 0.5
+        return state
+    two.register_load_state_dict_pre_hook(before)
+    two.register_load_state_dict_pre_hook(lambda opt, state: seen.append("second") or None)
+    two.register_load_state_dict_post_hook(lambda opt: seen.append(("after", opt is two, int(opt.state[b]["step"]))))
+    saved = one.state_dict()
+    two.load_state_dict(saved)
+    assert seen == ["before", "second", ("after", True, 1)]
+    assert two.param_groups[0]["lr"] == 0.5 and saved["param_groups"][0]["lr"] == 1e-3
+    handle = two.register_load_state_dict_pre_hook(lambda opt, state: state.update(mark=1))
+    two.load_state_dict(saved)
+    assert "mark" not in saved                                              # (a hook gets a dict of its own)
+    handle.remove()
+    assert torch.equal(two.state[b]["exp_avg"], one.state[a]["exp_avg"])
+
+
 # --------------------------------------------------------------------------- derivatives and traces that would be lost
 @pytest.mark.parametrize("name", ["layer_norm", "rotary", "cross_attention"])
 @pytest.mark.parametrize("plain", [True, False])

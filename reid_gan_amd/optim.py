@@ -6,6 +6,7 @@ tensors, as on the drop-in module route; the fused TrainStep has its own update 
 from __future__ import annotations
 
 from array import array
+from copy import deepcopy
 from operator import is_
 from typing import Dict, List, Tuple
 
@@ -205,8 +206,8 @@ class AdamW(torch.optim.Optimizer):
         return [bank.flat for gi, group in enumerate(self.param_groups) for bank in self._group_banks(gi, group)]
 
     def load_state_dict(self, state_dict):
-        """Copies the saved moments into this optimizer's buffers (so a captured step goes on with them); registered hooks run
-        before and after."""
+        """Copies the saved moments into this optimizer's buffers (so a captured step goes on with them), and all entries of the
+        groups but their parameters; registered hooks run before and after."""
         state_dict = dict(state_dict)                             # (a hook may change its own)
         for hook in self._optimizer_load_state_dict_pre_hooks.values():
             changed = hook(self, state_dict)
@@ -219,10 +220,11 @@ class AdamW(torch.optim.Optimizer):
             if theirs.get("state_bits", 32) != mine["state_bits"]:
                 raise ValueError(f"AdamW: a state of {theirs.get('state_bits', 32)} bits for an optimizer of {mine['state_bits']}")
             self._check_values(theirs["lr"], theirs["betas"], theirs["eps"], theirs["weight_decay"])
+            if theirs.get("maximize") or theirs.get("amsgrad"):
+                raise ValueError("AdamW: there is no maximize and no amsgrad")
         for gi, (mine, theirs) in enumerate(zip(self.param_groups, groups)):
-            for key in ("lr", "betas", "eps", "weight_decay", "initial_lr"):
-                if key in theirs:
-                    mine[key] = tuple(theirs[key]) if key == "betas" else theirs[key]
+            mine.update((key, deepcopy(value)) for key, value in theirs.items() if key not in ("params", "state_bits"))
+            mine["betas"] = tuple(mine["betas"])
             self._group_banks(gi, mine)
             for index, p in zip(theirs["params"], mine["params"]):
                 views, saved = self.state[p], state_dict["state"].get(index)

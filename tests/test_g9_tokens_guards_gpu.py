@@ -108,6 +108,25 @@ def test_adamw_load_state_dict_runs_its_hooks():
     assert torch.equal(two.state[b]["exp_avg"], one.state[a]["exp_avg"])
 
 
+def test_adamw_group_entries_travel():
+    """What a schedule or a caller keeps in the groups comes back with them, as with every torch optimizer."""
+    a, b = ones(5), ones(5)
+    one = optim.AdamW([{"params": [a], "name": "decoder"}])
+    sched = torch.optim.lr_scheduler.OneCycleLR(one, max_lr=0.1, total_steps=50)
+    for _ in range(7):
+        one.step(), sched.step()
+    saved = copy.deepcopy(one.state_dict())
+    two = optim.AdamW([{"params": [b], "name": "?"}])
+    torch.optim.lr_scheduler.OneCycleLR(two, max_lr=9.0, total_steps=50)
+    two.load_state_dict(saved)
+    mine = two.param_groups[0]
+    assert mine["params"][0] is b
+    assert {k: v for k, v in mine.items() if k != "params"} == {k: v for k, v in saved["param_groups"][0].items() if k != "params"}
+    assert mine["name"] == "decoder" and mine["max_lr"] == 0.1
+    saved["param_groups"][0]["name"] = "other"                              # (nothing is shared with what was loaded)
+    assert mine["name"] == "decoder"
+
+
 # --------------------------------------------------------------------------- derivatives and traces that would be lost
 @pytest.mark.parametrize("name", ["layer_norm", "rotary", "cross_attention"])
 @pytest.mark.parametrize("plain", [True, False])

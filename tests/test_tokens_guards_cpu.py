@@ -5,7 +5,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from reid_gan_amd import _lib, attention
+from reid_gan_amd import _lib, attention, optim
 
 BF16 = torch.bfloat16
 
@@ -72,3 +72,12 @@ def test_cross_attention_takes_small_scales():
     call, args = calls()["cross_attention"]
     with pytest.raises(RuntimeError, match="no CPU path"):
         call(*args, scale=1e-36)
+
+
+@pytest.mark.parametrize("entry", ["maximize", "amsgrad"])
+def test_adamw_refuses_states_of_another_update(entry):
+    """A torch state whose groups ask for an update that is not this one's."""
+    p = torch.nn.Parameter(torch.zeros(4))
+    saved = torch.optim.AdamW([p], **{entry: True}).state_dict()
+    with pytest.raises(ValueError, match="no maximize and no amsgrad"):
+        optim.AdamW([p]).load_state_dict(saved)

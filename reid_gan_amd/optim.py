@@ -179,17 +179,17 @@ class AdamW(torch.optim.Optimizer):
         if kinds and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: run a step before the capture")
         banks = [_Bank(ps, group["state_bits"]) for ps in kinds.values()]
+        states = [(p, views) for bank in banks for p, views in zip(bank.params, bank.views())]
+        for p, views in states:
+            if self.state.get(p):
+                self._check_state(self.state[p], views)
+                self._take(self.state[p], views)
+        self.state.update(states)
         self._banks[gi] = list(group["params"]), banks
-        for bank in banks:
-            for p, views in zip(bank.params, bank.views()):
-                saved = self.state.get(p)
-                if saved:
-                    self._take(saved, views)
-                self.state[p] = views
         return banks
 
     @staticmethod
-    def _take(saved, views):
+    def _check_state(saved, views):
         if set(saved) != set(views):
             raise ValueError(f"AdamW: state with {sorted(saved)}, wanted {sorted(views)} (moments of another number of bits?)")
         for name, dst in views.items():
@@ -198,7 +198,11 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"AdamW: state `{name}` has shape {tuple(src.shape)}, not {tuple(dst.shape)}")
             if name != "step" and (src.dtype is CODES) != (dst.dtype is CODES):
                 raise ValueError(f"AdamW: state `{name}` is {src.dtype}, not {dst.dtype}")
-            dst.copy_(src.reshape(dst.shape))
+
+    @staticmethod
+    def _take(saved, views):
+        for name, dst in views.items():
+            dst.copy_(torch.as_tensor(saved[name]).reshape(dst.shape))
 
     def flat_state(self) -> List[Dict[str, torch.Tensor]]:
         """The moments of all tensors in one buffer per kind - one dict per group and element type, in the order of the
@@ -207,7 +211,7 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Copies the saved moments into this optimizer's buffers (so a captured step goes on with them), and all entries of the
-        groups but their parameters; registered hooks run before and after."""
+        groups but their parameters; registered hooks run before and after.  A state that does not fit changes nothing."""
         state_dict = dict(state_dict)                             # (a hook may change its own)
         for hook in self._optimizer_load_state_dict_pre_hooks.values():
             changed = hook(self, state_dict)
@@ -222,17 +226,22 @@ class AdamW(torch.optim.Optimizer):
             self._check_values(theirs["lr"], theirs["betas"], theirs["eps"], theirs["weight_decay"])
             if theirs.get("maximize") or theirs.get("amsgrad"):
                 raise ValueError("AdamW: there is no maximize and no amsgrad")
-        for gi, (mine, theirs) in enumerate(zip(self.param_groups, groups)):
+        for gi, mine in enumerate(self.param_groups):
+            self._group_banks(gi, mine)
+        states = [(state_dict["state"].get(index), self.state[p])
+                  for mine, theirs in zip(self.param_groups, groups) for index, p in zip(theirs["params"], mine["params"])]
+        for saved, views in states:                               # (everything is looked at before anything is written)
+            if saved:
+                self._check_state(saved, views)
+        for mine, theirs in zip(self.param_groups, groups):
             mine.update((key, deepcopy(value)) for key, value in theirs.items() if key not in ("params", "state_bits"))
             mine["betas"] = tuple(mine["betas"])
-            self._group_banks(gi, mine)
-            for index, p in zip(theirs["params"], mine["params"]):
-                views, saved = self.state[p], state_dict["state"].get(index)
-                if saved:
-                    self._take(saved, views)
-                else:
-                    for t in views.values():
-                        (t.view(torch.uint8) if t.dtype is CODES else t).zero_()
+        for saved, views in states:
+            if saved:
+                self._take(saved, views)
+            else:
+                for t in views.values():
+                    (t.view(torch.uint8) if t.dtype is CODES else t).zero_()
         for hook in self._optimizer_load_state_dict_post_hooks.values():
             hook(self)
 

@@ -127,6 +127,31 @@ def test_adamw_group_entries_travel():
     assert mine["name"] == "decoder"
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_a_refused_state_changes_nothing(bits):
+    a, b = ones(300), ones(40)
+    opt = optim.AdamW([{"params": [a]}, {"params": [b], "lr": 0.25}], state_bits=bits)
+    opt.step()
+    good = copy.deepcopy(opt.state_dict())
+    a.grad.mul_(3), opt.step()
+    held = copy.deepcopy(opt.state_dict())
+    shape, names, kind, value, group = (copy.deepcopy(good) for _ in range(5))
+    shape["state"][1]["exp_avg"] = shape["state"][1]["exp_avg"][:3]
+    names["state"][1]["max_exp_avg_sq"] = names["state"][1]["exp_avg"]
+    kind["state"][1]["exp_avg"] = torch.zeros(40, device=DEV, dtype=F32 if bits == 8 else torch.float8_e4m3fn)
+    value["param_groups"][1]["lr"] = -1.0
+    group["param_groups"][1]["maximize"] = True
+    for i, bad in enumerate((shape, names, kind, value, group)):
+        bad["param_groups"][0]["lr"] = 77.0
+        with pytest.raises(ValueError):
+            opt.load_state_dict(bad)
+        now = opt.state_dict()
+        assert now["param_groups"] == held["param_groups"], i
+        for s in (0, 1):
+            for name, t in held["state"][s].items():
+                assert torch.equal(now["state"][s][name].float(), t.float()), (i, s, name)
+
+
 # --------------------------------------------------------------------------- derivatives and traces that would be lost
 @pytest.mark.parametrize("name", ["layer_norm", "rotary", "cross_attention"])
 @pytest.mark.parametrize("plain", [True, False])

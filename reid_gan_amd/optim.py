@@ -8,7 +8,7 @@ from __future__ import annotations
 from array import array
 from copy import deepcopy
 from operator import is_
-from typing import Dict, List, Tuple
+from typing import Dict, List, Optional, Tuple
 
 import torch
 
@@ -52,7 +52,9 @@ class _Bank:
                 for name in ("exp_avg", "exp_avg_sq_root"):
                     self.flat[name] = torch.zeros(many, dtype=torch.uint8, device=self.device).view(CODES)
                     self.flat[name + "_scale"] = torch.zeros(many // BLOCK, dtype=F32, device=self.device)
-        self.tables: List[torch.Tensor] = []          # (earlier ones stay: a captured graph may hold their address)
+        self.table: Optional[torch.Tensor] = None
+        self.captured = False                         # whether a captured step reads the table
+        self.kept: List[torch.Tensor] = []            # earlier tables that one reads
         self.at = array("q")
         self.elements = array("q", self.sizes)
         self.grads = array("q", bytes(8 * len(params)))
@@ -88,7 +90,13 @@ class _Bank:
         ms, vs = (self.flat[k].data_ptr() for k in self.flat if k.endswith("_scale")) if self.bits == 8 else (0, 0)
         rows = [(p, m + s * one, v + s * one, ms and ms + s // BLOCK * 4, vs and vs + s // BLOCK * 4, n)
                 for p, s, n in zip(at, self.starts, self.sizes)]
-        self.tables.append(torch.tensor(rows, dtype=torch.int64).to(self.device))
+        rows = torch.tensor(rows, dtype=torch.int64)
+        if self.table is None or self.captured:
+            if self.captured:
+                self.kept.append(self.table)
+            self.table, self.captured = rows.to(self.device), False
+        else:                                                     # (on the stream of this step, so behind the one before it)
+            self.table.copy_(rows)
         self.at = at
 
     def gradients(self):
@@ -254,6 +262,7 @@ class AdamW(torch.optim.Optimizer):
         for gi, group in enumerate(self.param_groups):
             for bank in self._group_banks(gi, group):
                 kept = bank.gradients()                            # noqa: F841  (alive until the launch)
-                ops.adamw_jobs(bank.tables[-1], bank.map, bank.grads, bank.first, bank.steps, bank.coef, float(group["lr"]),
+                bank.captured |= torch.cuda.is_current_stream_capturing()
+                ops.adamw_jobs(bank.table, bank.map, bank.grads, bank.first, bank.steps, bank.coef, float(group["lr"]),
                                group["betas"][0], group["betas"][1], group["eps"], group["weight_decay"], bank.dtype, bank.bits)
         return loss

@@ -82,6 +82,43 @@ def test_adamw_refuses_a_parameter_that_was_transposed_where_it_lies():
     opt.step()
 
 
+def test_adamw_parameters_that_move_at_every_step_cost_no_memory():
+    ps = [ones(3) for _ in range(900)]                                      # (a job table of 43 KB)
+    opt = optim.AdamW(ps)
+    homes = [[p.data for p in ps], [p.data.clone() for p in ps]]
+    for i in range(40):
+        for p, t in zip(ps, homes[i & 1]):
+            p.data = t
+        opt.step()
+        if i == 3:
+            base = torch.cuda.memory_allocated()
+    assert torch.cuda.memory_allocated() <= base + 8192
+
+
+def test_adamw_a_captured_step_keeps_its_table_when_parameters_move():
+    """Parameters move away after a capture and come back: the replays go on where the capture found them."""
+    a, b = ones(700), ones(700)
+    one, two = optim.AdamW([a], lr=1e-2), optim.AdamW([b], lr=1e-2)
+    one.step(), two.step()
+    graph = torch.cuda.CUDAGraph()
+    GRAPHS.append(graph)
+    with torch.cuda.graph(graph):
+        one.step()
+    home = a.data
+    for i in range(3):
+        a.data = home.clone()
+        for _ in range(3):                                                  # (and tables are made for other places)
+            a.data = a.data.clone()
+            one.step(), two.step()
+        home.copy_(a.data)
+        a.data = home
+        graph.replay(), two.step()
+        torch.cuda.synchronize()
+        assert torch.equal(a, b), i
+        one.step(), two.step()
+        assert torch.equal(a, b), i
+
+
 # --------------------------------------------------------------------------- AdamW: state dicts
 def test_adamw_load_state_dict_runs_its_hooks():
     a, b = ones(5), ones(5)

@@ -758,6 +758,12 @@ def _on_device(t: torch.Tensor, entry, *args):
             entry(*args, _raw_stream(index))
 
 
+def _buffers(first: torch.Tensor, *others, floats=()):
+    """The kernels take addresses: every tensor lies on the device of the first, and scratch (`floats`) holds fp32."""
+    assert first.is_cuda and all(t is None or t.device == first.device for t in (*others, *floats)), "tensors on one ROCm device"
+    assert all(t is None or (t.dtype is torch.float32 and t.is_contiguous()) for t in floats), "scratch in contiguous fp32"
+
+
 def _row_stride(t: torch.Tensor) -> int:
     return t.shape[-1] if t.is_contiguous() else t.stride(0)
 
@@ -768,9 +774,10 @@ def layer_norm_fwd(x: torch.Tensor, w, b, y: torch.Tensor, stats, eps: float):
     C, wt = x.shape[-1], w if w is not None else b
     rows = x.numel() // C
     assert y.numel() == x.numel() and y.shape[-1] == C and y.dtype is x.dtype
-    assert all(t is None or (t.numel() == C and t.is_contiguous()) for t in (w, b))
+    assert all(t is None or (t.numel() == C and t.is_contiguous() and t.dtype is wt.dtype) for t in (w, b))
     assert all(t.is_contiguous() or (t.dim() == 2 and (C == 1 or t.stride(1) == 1)) for t in (x, y))
-    assert stats is None or (stats.dtype is torch.float32 and stats.is_contiguous() and stats.numel() == 2 * rows)
+    assert stats is None or stats.numel() == 2 * rows
+    _buffers(x, w, b, y, floats=(stats,))
     at = 0 if stats is None else stats.data_ptr()
     _on_device(x, lib.ried_layer_norm_fwd, x.data_ptr(), _row_stride(x), _p(w), _p(b), y.data_ptr(), _row_stride(y), at or None,
                at + 4 * rows if at else None, rows, C, eps, TOKEN_TYPES[x.dtype], 0 if wt is None else TOKEN_TYPES[wt.dtype])
@@ -789,8 +796,9 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, w, stats: torch.Tensor, dx
     assert dy.numel() == dx.numel() == x.numel() and dy.dtype is dx.dtype is x.dtype and dy.shape[-1] == dx.shape[-1] == C
     assert all(t.is_contiguous() or (t.dim() == 2 and (C == 1 or t.stride(1) == 1)) for t in (x, dy, dx))
     assert all(t is None or (t.numel() == C and t.is_contiguous() and t.dtype is wt.dtype) for t in (w, dw, db))
-    assert stats.dtype is torch.float32 and stats.is_contiguous() and stats.numel() == 2 * rows
+    assert stats.numel() == 2 * rows
     assert (dw is None and db is None) or scratch.numel() >= layer_norm_bwd_scratch_floats(rows, C, x.dtype)
+    _buffers(x, dy, w, dx, dw, db, floats=(stats, scratch))
     at = stats.data_ptr()
     _on_device(x, lib.ried_layer_norm_bwd, dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x), _p(w), at, at + 4 * rows,
                dx.data_ptr(), _row_stride(dx), _p(dw), _p(db), _p(scratch), rows, C, TOKEN_TYPES[x.dtype],
@@ -804,6 +812,7 @@ def rotary(x: torch.Tensor, y: torch.Tensor, positions: torch.Tensor, freqs: tor
     assert y.shape == x.shape and y.dtype is x.dtype and (D == 1 or x.stride(3) == y.stride(3) == 1)
     assert positions.shape == (B, L, len(sections)) and freqs.dtype is torch.float64 and freqs.is_contiguous()
     assert freqs.numel() == sum(sections)
+    _buffers(x, y, positions, freqs)
     s = tuple(sections) + (0,) * (4 - len(sections))
     xs, ys, ps = x.stride(), y.stride(), positions.stride()
     _on_device(x, lib.ried_rotary, x.data_ptr(), xs[0], xs[1], xs[2], y.data_ptr(), ys[0], ys[1], ys[2],
@@ -841,10 +850,11 @@ def _xattn_check(q, k, v, out, lse, lengths, key_mask, scratch, floats: int):
     (B, Lq, H, _), Lk = q.shape, k.shape[1]
     assert k.shape == v.shape and k.shape[0] == B and k.shape[3] == q.shape[3] and out.shape == q.shape
     assert q.dtype is k.dtype is v.dtype is out.dtype and all(t.shape[3] == 1 or t.stride(3) == 1 for t in (q, k, v, out))
-    assert lse is None or (lse.dtype is torch.float32 and lse.is_contiguous() and lse.numel() == B * H * Lq)
+    assert lse is None or lse.numel() == B * H * Lq
     assert lengths is None or (lengths.dtype is torch.int32 and lengths.is_contiguous() and lengths.numel() == B)
     assert key_mask is None or (key_mask.element_size() == 1 and key_mask.shape == (B, Lk) and (Lk < 2 or key_mask.stride(1) == 1))
-    assert floats == 0 or (scratch.dtype is torch.float32 and scratch.is_contiguous() and scratch.numel() >= floats)
+    assert floats == 0 or scratch.numel() >= floats
+    _buffers(q, k, v, out, lengths, key_mask, floats=(lse, scratch))
 
 
 def xattn_fwd(q, k, v, out, lse, scale: float, lengths=None, key_mask=None, scratch=None):
@@ -861,6 +871,7 @@ def xattn_bwd(dout, q, k, v, out, lse, dq, dk, dv, scale: float, scratch, length
     _xattn_check(q, k, v, out, lse, lengths, key_mask, scratch, xattn_bwd_scratch_floats(B, Lq, Lk, H, G, D))
     assert lse is not None and dout.shape == dq.shape == q.shape and dk.shape == dv.shape == k.shape
     assert all(t.dtype is q.dtype and (D == 1 or t.stride(3) == 1) for t in (dout, dq, dk, dv))
+    _buffers(q, dout, dq, dk, dv)
     _on_device(q, lib.ried_xattn_bwd, _xattn_desc(q, k, v, out, lse, lengths, key_mask, scratch, scale, dout, dq, dk, dv))
 
 

@@ -287,3 +287,19 @@ def test_cross_attention_small_scales_keep_hidden_keys_out():
     for scale in (1e-46, 1e30):
         with pytest.raises(ValueError, match="scale"):
             attention.cross_attention(q, k, v, key_mask=mask, scale=scale)
+
+
+# --------------------------------------------------------------------------- functions on buffers
+@pytest.mark.parametrize("name", ["layer_norm_fwd", "layer_norm_bwd", "rotary", "xattn_fwd", "xattn_bwd"])
+def test_functions_on_buffers_refuse_what_the_kernels_could_not_read(name):
+    """Refused before any launch: one tensor in host memory, scratch and statistics of another type."""
+    from test_tokens_guards_cpu import buffer_calls
+    call, tensors = buffer_calls(DEV)[name]
+    call(**tensors)
+    for one in tensors:
+        with pytest.raises(AssertionError):
+            call(**{**tensors, one: tensors[one].cpu()})
+    for one in set(tensors) & {"stats", "scratch", "lse"}:
+        with pytest.raises(AssertionError):
+            call(**{**tensors, one: tensors[one].to(BF16)})
+    torch.cuda.synchronize()

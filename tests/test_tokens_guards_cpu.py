@@ -5,7 +5,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from reid_gan_amd import _lib, attention, optim
+from reid_gan_amd import _lib, attention, ops, optim
 
 BF16 = torch.bfloat16
 
@@ -81,3 +81,37 @@ def test_adamw_refuses_states_of_another_update(entry):
     saved = torch.optim.AdamW([p], **{entry: True}).state_dict()
     with pytest.raises(ValueError, match="no maximize and no amsgrad"):
         optim.AdamW([p]).load_state_dict(saved)
+
+
+def buffer_calls(device):
+    """name: (function of its tensors, the tensors by name) of the functions on buffers"""
+    z = lambda *shape, to=BF16: torch.zeros(*shape, dtype=to, device=device)
+    F32 = torch.float32
+    rows = dict(x=z(4, 64), w=z(64, to=F32), b=z(64, to=F32), y=z(4, 64), stats=z(2, 4, to=F32))
+    back = dict(dy=z(4, 64), x=z(4, 64), w=z(64, to=F32), stats=z(2, 4, to=F32), dx=z(4, 64), dw=z(64, to=F32), db=z(64, to=F32),
+                scratch=z(4096, to=F32))
+    turn = dict(x=z(1, 3, 2, 8), y=z(1, 3, 2, 8), pos=z(1, 3, 1, to=F32), freqs=z(4, to=torch.float64))
+    some = dict(q=z(1, 2, 2, 64), k=z(1, 4, 2, 64), v=z(1, 4, 2, 64), out=z(1, 2, 2, 64), lse=z(1, 2, 2, to=F32),
+                lengths=z(1, to=torch.int32), mask=z(1, 4, to=torch.bool), scratch=z(4096, to=F32))
+    grads = dict(some, dout=z(1, 2, 2, 64), dq=z(1, 2, 2, 64), dk=z(1, 4, 2, 64), dv=z(1, 4, 2, 64))
+    return {"layer_norm_fwd": (lambda x, w, b, y, stats: ops.layer_norm_fwd(x, w, b, y, stats, 1e-5), rows),
+            "layer_norm_bwd": (lambda **t: ops.layer_norm_bwd(**t), back),
+            "rotary": (lambda x, y, pos, freqs: ops.rotary(x, y, pos, freqs, (4,), False, False), turn),
+            "xattn_fwd": (lambda q, k, v, out, lse, lengths, mask, scratch: ops.xattn_fwd(q, k, v, out, lse, 0.125, lengths, mask, scratch), some),
+            "xattn_bwd": (lambda q, k, v, out, lse, lengths, mask, scratch, dout, dq, dk, dv:
+                          ops.xattn_bwd(dout, q, k, v, out, lse, dq, dk, dv, 0.125, scratch, lengths, mask), grads)}
+
+
+@pytest.mark.parametrize("name", list(buffer_calls("cpu")))
+def test_functions_on_buffers_refuse_host_memory(name):
+    call, tensors = buffer_calls("cpu")[name]
+    with pytest.raises(AssertionError, match="ROCm device"):
+        call(**tensors)
+
+
+def test_layer_norm_on_buffers_refuses_parameters_of_two_types():
+    call, tensors = buffer_calls("cpu")["layer_norm_fwd"]
+    for name in ("w", "b"):
+        with pytest.raises(AssertionError) as error:
+            call(**{**tensors, name: tensors[name].to(BF16)})
+        assert "ROCm" not in str(error.value)

@@ -280,6 +280,14 @@ def _laid_out(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=_CONTIGUOUS)
 
 
+def _near(t: torch.Tensor, share: int) -> torch.Tensor:
+    """t laid out, and the heads that share a key head (`share` of them) within 2^31 bytes, as the gradients' kernels read q and
+    dout."""
+    t = _laid_out(t)
+    far = (t.shape[1] * t.stride(1) + share * t.stride(2)) * 2 >= 1 << 31
+    return t.clone(memory_format=_CONTIGUOUS) if far else t
+
+
 def _attend(q, k, v, lengths, key_mask, scale, lse):
     (B, Lq, H, D), (_, Lk, G, _) = q.shape, k.shape
     out = torch.empty_like(q, memory_format=_CONTIGUOUS)
@@ -292,7 +300,7 @@ class _CrossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, key_mask, scale):
         _not_captured("cross_attention")
-        q, k, v = _laid_out(q), _laid_out(k), _laid_out(v)
+        q, k, v = _near(q, q.shape[2] // k.shape[2]), _laid_out(k), _laid_out(v)
         B, Lq, H, _ = q.shape
         lse = q.new_empty((B, H, Lq), dtype=F32)
         out = _attend(q, k, v, lengths, key_mask, scale, lse)
@@ -310,7 +318,7 @@ class _CrossFn(torch.autograd.Function):
         if Lq == 0:
             return dq, dk.zero_(), dv.zero_(), None, None, None
         scratch = lse.new_empty((ops.xattn_bwd_scratch_floats(B, Lq, Lk, H, G, D),))
-        ops.xattn_bwd(_laid_out(dout), q, k, v, out, lse, dq, dk, dv, ctx.scale, scratch, lengths, key_mask)
+        ops.xattn_bwd(_near(dout, H // G), q, k, v, out, lse, dq, dk, dv, ctx.scale, scratch, lengths, key_mask)
         return dq, dk, dv, None, None, None
 
 
@@ -323,7 +331,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: 
     count; key_mask: bool or uint8 [batch][keys], nonzero keys count; with both, keys that both allow.  An entry without
     keys gives zeros and no gradient; hidden keys have no effect whatever they hold, and get zero gradients.  scale:
     channels ** -0.5 unless given (between 1e-37 and 1e30).  channels: a multiple of 8 up to 128, bf16 or fp16.  Views are
-    read where they lie when their channels are adjacent and their strides are multiples of 8 elements; others are copied."""
+    read where they lie when their channels are adjacent and their strides are multiples of 8 elements; others are copied.
+    With gradients, the queries of an entry are under 2^31 bytes."""
     o = direct().cross_attention(q, k, v, lengths, key_mask, scale)
     if o is not None:
         return o
@@ -354,7 +363,11 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: 
     scale = D ** -0.5 if scale is None else float(scale)
     if not 1e-37 < scale < 1e30:
         raise ValueError("cross_attention: scale is a positive number between 1e-37 and 1e30")
+    wanted = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    if wanted and (qs[1] * H * D + H // ks[2] * D) * 2 >= 1 << 31:
+        raise ValueError(f"cross_attention: gradients of {qs[1]} queries of {H} x {D} channels (2^31 bytes or more an entry) are not "
+                         "taken; pass fewer queries")
     _on_gpu("cross_attention", q)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if wanted:
         return _CrossFn.apply(q, k, v, lengths, key_mask, scale)
     return _attend(_laid_out(q), _laid_out(k), _laid_out(v), lengths, key_mask, scale, None)

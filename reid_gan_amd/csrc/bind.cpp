@@ -177,6 +177,8 @@ bool laid_out(const Tensor& t) {
   return s[3] == 1 && ((s[0] | s[1] | s[2]) & 7) == 0 && s[0] >= 0 && s[1] >= 0 && s[1] <= (1 << 23) && s[2] >= 0 &&
          (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0;
 }
+// The gradients' kernels reach the heads that share a key head (`share` of them) by 32-bit offsets in q and in dout.
+bool far(const Tensor& t, int64_t share) { return (t.size(1) * t.stride(1) + share * t.stride(2)) * 2 >= (1ll << 31); }
 void strides(long long (&to)[3], const Tensor& t) {
   for (int i = 0; i < 3; ++i) to[i] = t.stride(i);
 }
@@ -227,7 +229,8 @@ struct Cross : torch::autograd::Function<Cross> {
       dk.zero_();
       dv.zero_();
     } else {
-      Tensor dout = laid_out(grads[0]) ? grads[0] : grads[0].clone(at::MemoryFormat::Contiguous);
+      const bool there = laid_out(grads[0]) && !far(grads[0], q.size(2) / k.size(2));
+      Tensor dout = there ? grads[0] : grads[0].clone(at::MemoryFormat::Contiguous);
       ried_xattn_t d = attention(q, k, v, o, lse, saved[5], saved[6], ctx->saved_data["scale"].toDouble());
       d.dout = address(dout);
       d.dq = dq.mutable_data_ptr(); d.dk = dk.mutable_data_ptr(); d.dv = dv.mutable_data_ptr();
@@ -353,7 +356,7 @@ PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (dual(q) || dual(k) || dual(v)) Py_RETURN_NONE;
   c10::DeviceGuard guard(q.device());
   if (!wanted({&q, &k, &v})) return THPVariable_Wrap(attend(q, k, v, Tensor(), lengths, mask, scale));
-  if (capturing(q)) Py_RETURN_NONE;
+  if (capturing(q) || far(q, q.size(2) / k.size(2))) Py_RETURN_NONE;
   return THPVariable_Wrap(Cross::apply(q, k, v, Keys{lengths, mask}, scale));
   END_HANDLE_TH_ERRORS
 }

@@ -303,3 +303,20 @@ def test_functions_on_buffers_refuse_what_the_kernels_could_not_read(name):
         with pytest.raises(AssertionError):
             call(**{**tensors, one: tensors[one].to(BF16)})
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("plain", [True, False])
+def test_cross_attention_gradients_where_queries_lie_far_apart(plain):
+    """Views of q and of the incoming gradient that span over 2^31 bytes: the kernels of the gradients get copies."""
+    wrap = (lambda t: t) if plain else (lambda t: t.as_subclass(Sub))
+    big = torch.empty(600 << 22, dtype=BF16, device=DEV)
+    q, d = (big.as_strided((1, 600, 4, 64), (0, 1 << 22, 64, 1), at) for at in (0, 4096))
+    q.copy_(normal(30, 1, 600, 4, 64)), d.copy_(normal(31, 1, 600, 4, 64))
+    k, v = normal(32, 1, 77, 2, 64, to=BF16), normal(33, 1, 77, 2, 64, to=BF16)
+    results = []
+    for a, g in ((q, d), (q, d.contiguous()), (q.contiguous(), d), (q.contiguous(), d.contiguous())):
+        leaves = [t.detach().requires_grad_() for t in (a, k, v)]
+        out = attention.cross_attention(*map(wrap, leaves))
+        results.append([out.detach().as_subclass(torch.Tensor), *torch.autograd.grad(out, leaves, g)])
+    for got in results[:3]:
+        assert all(torch.equal(a, b.as_subclass(torch.Tensor)) for a, b in zip(results[3], got))

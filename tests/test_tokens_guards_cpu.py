@@ -115,3 +115,10 @@ def test_layer_norm_on_buffers_refuses_parameters_of_two_types():
         with pytest.raises(AssertionError) as error:
             call(**{**tensors, name: tensors[name].to(BF16)})
         assert "ROCm" not in str(error.value)
+
+
+def test_cross_attention_refuses_gradients_of_too_many_queries_before_it_works_on_them():
+    meta = lambda n: torch.zeros(1, n, 16, 128, dtype=BF16, device="meta")
+    for q, error in ((meta(1 << 19), "fewer queries"), (meta((1 << 19) - 1), "no CPU path")):
+        with pytest.raises((ValueError, RuntimeError), match=error):
+            attention.cross_attention(q.requires_grad_(), meta(77), meta(77))

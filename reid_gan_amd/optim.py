@@ -259,10 +259,10 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for gi, group in enumerate(self.param_groups):
-            for bank in self._group_banks(gi, group):
-                kept = bank.gradients()                            # noqa: F841  (alive until the launch)
-                bank.captured |= torch.cuda.is_current_stream_capturing()
-                ops.adamw_jobs(bank.table, bank.map, bank.grads, bank.first, bank.steps, bank.coef, float(group["lr"]),
-                               group["betas"][0], group["betas"][1], group["eps"], group["weight_decay"], bank.dtype, bank.bits)
+        work = [(group, bank) for gi, group in enumerate(self.param_groups) for bank in self._group_banks(gi, group)]
+        kept = [bank.gradients() for _, bank in work]              # noqa: F841  (alive until the launches; all refusals come first)
+        for group, bank in work:
+            bank.captured |= torch.cuda.is_current_stream_capturing()
+            ops.adamw_jobs(bank.table, bank.map, bank.grads, bank.first, bank.steps, bank.coef, float(group["lr"]),
+                           group["betas"][0], group["betas"][1], group["eps"], group["weight_decay"], bank.dtype, bank.bits)
         return loss

@@ -320,3 +320,24 @@ def test_cross_attention_gradients_where_queries_lie_far_apart(plain):
         results.append([out.detach().as_subclass(torch.Tensor), *torch.autograd.grad(out, leaves, g)])
     for got in results[:3]:
         assert all(torch.equal(a, b.as_subclass(torch.Tensor)) for a, b in zip(results[3], got))
+
+
+def test_adamw_a_refused_step_changes_nothing():
+    """A second group's parameter or gradient that cannot be taken: the first group is not stepped either."""
+    def moved(p, q):
+        q.data = q.data.new_zeros(9)
+
+    def wrong(p, q):
+        q.grad = torch.sparse_coo_tensor([[0]], [1.0], (7,), device=DEV)
+
+    def replaced(p, q):
+        opt.param_groups[1]["params"] = [ones(7)]
+    for break_it in (moved, wrong, replaced):
+        p, q = ones(300), ones(7)
+        opt = optim.AdamW([{"params": [p]}, {"params": [q]}])
+        opt.step()
+        before, count = p.detach().clone(), int(opt.state[p]["step"])
+        break_it(p, q)
+        with pytest.raises((RuntimeError, TypeError, ValueError)):
+            opt.step()
+        assert torch.equal(p, before) and int(opt.state[p]["step"]) == count == 1

@@ -4,8 +4,7 @@
 // (C1 = (0.01*range)^2, C2 = (0.03*range)^2 on values clamped to [-160, 240], src/test.py:77-80).
 // The reference launches five 11x11 convolutions and ~15 elementwise ops per image pair; here one
 // kernel stages a 42x42 halo tile per image in LDS, runs the 11-tap Gaussian separably
-// (horizontal pass into LDS, vertical pass in registers, both on pairs of quantities through
-// packed fp32 FMAs), forms the SSIM quotient with the same
+// (horizontal pass into LDS, vertical pass in registers, both on pairs of quantities), forms the SSIM quotient with the same
 // sigma = E[x^2] - mu^2 algebra and reduces with wavefront shuffles.  fp32 throughout: the
 // variance cancellation on raw HU makes bf16 unusable here.
 //

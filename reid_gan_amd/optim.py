@@ -161,6 +161,10 @@ class AdamW(torch.optim.Optimizer):
     def _check_values(lr, betas, eps, weight_decay):
         if isinstance(lr, torch.Tensor):
             raise TypeError("AdamW: lr is a number, not a tensor")
+        AdamW._check_numbers(lr, betas, eps, weight_decay)
+
+    @staticmethod
+    def _check_numbers(lr, betas, eps, weight_decay):
         if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1):
             raise ValueError("AdamW: lr, eps and weight_decay are not negative, betas lie in [0, 1)")
 
@@ -259,6 +263,8 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        for group in self.param_groups:
+            self._check_numbers(group["lr"], group["betas"], group["eps"], group["weight_decay"])
         work = [(group, bank) for gi, group in enumerate(self.param_groups) for bank in self._group_banks(gi, group)]
         kept = [bank.gradients() for _, bank in work]              # noqa: F841  (alive until the launches; all refusals come first)
         for group, bank in work:

@@ -323,7 +323,7 @@ def test_cross_attention_gradients_where_queries_lie_far_apart(plain):
 
 
 def test_adamw_a_refused_step_changes_nothing():
-    """A second group's parameter or gradient that cannot be taken: the first group is not stepped either."""
+    """A second group's parameter, gradient or rate that cannot be taken: the first group is not stepped either."""
     def moved(p, q):
         q.data = q.data.new_zeros(9)
 
@@ -332,7 +332,10 @@ def test_adamw_a_refused_step_changes_nothing():
 
     def replaced(p, q):
         opt.param_groups[1]["params"] = [ones(7)]
-    for break_it in (moved, wrong, replaced):
+
+    def negative(p, q):
+        opt.param_groups[1]["lr"] = -1.0
+    for break_it in (moved, wrong, replaced, negative):
         p, q = ones(300), ones(7)
         opt = optim.AdamW([{"params": [p]}, {"params": [q]}])
         opt.step()

@@ -2,7 +2,7 @@
 
 There is no network for checkpoints or datasets, so parity tests and the
 benchmark regenerate every state dict from a seed.  numpy's PCG64 stream is
-used (not torch's RNG) so that the build container and the GPU box produce
+used (not torch's RNG) so that machines with and without a GPU produce
 identical values.  Pure numpy/torch-CPU; no GPU code here.
 """
 from __future__ import annotations

@@ -1,5 +1,5 @@
 #!/bin/bash
-# Collect the round's profile evidence on the GPU box (run from the repository root through gpurun):
+# Collect the profiles (run from the repository root on a machine with the GPU):
 #   kernel traces of the training step and of the inference batch (per-kernel summary of the last repetition, timeline),
 #   three counter passes over the training step (MFMA busy; HBM fetch; HBM write), each in a run of its own.
 # Usage: tools/collect_profiles.sh <tag>   -> gpurun_out/<tag>_*.txt|json

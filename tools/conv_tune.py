@@ -1,4 +1,4 @@
-"""Time every distinct convolution of the training step under each tile configuration (run on the GPU box)."""
+"""Time every distinct convolution of the training step under each tile configuration."""
 import sys, os
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import torch

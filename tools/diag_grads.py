@@ -1,4 +1,4 @@
-"""Gradient diagnostics of the HIP plans against the (bf16-emulating) oracle; run on the GPU box."""
+"""Gradient diagnostics of the HIP plans against the (bf16-emulating) oracle; needs a GPU."""
 import sys, os
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import torch

@@ -1,4 +1,4 @@
-"""Per-layer error report of the HIP plans against the CPU oracle (run on the GPU box)."""
+"""Per-layer error report of the HIP plans against the CPU oracle."""
 import sys, os
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import torch

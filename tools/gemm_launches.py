@@ -1,4 +1,4 @@
-"""Per-launch table of the GEMM-family kernels in one eager training step (run on the GPU box)."""
+"""Per-launch table of the GEMM-family kernels in one eager training step."""
 import sys, os
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import torch

@@ -1,5 +1,5 @@
 #!/bin/bash
-# One SQ counter pass over the training step (run from the repository root through gpurun):
+# One SQ counter pass over the training step (run from the repository root on a machine with the GPU):
 #   tools/pmc_sq.sh <tag> <kernel patterns> <counter> [<counter> ...]   -> gpurun_out/<tag>.json
 set -u
 tag=$1; pat=$2; shift 2

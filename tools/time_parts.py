@@ -1,4 +1,4 @@
-"""Time G forward+backward, D forward+backward and VGG forward+backward alone (graph replays) on the GPU box."""
+"""Time G forward+backward, D forward+backward and VGG forward+backward alone (graph replays)."""
 import sys, os
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import torch
